@@ -84,12 +84,14 @@ def draw(rng):
     Hkv = rng.choice([1, 2, 3, 4, 8])
     G = rng.choice([1, 1, 2, 4, 5])
     if op.startswith("window"):
-        S = _log(rng, 1, 8192)
+        # A query that sees one key has dS = 0 and gradients of nothing but rounding.
+        bwd = op == "window_bwd"
+        S = _log(rng, 8 if bwd else 1, 8192)
         B = max(1, min(_log(rng, 1, 16), 4 * 8192 // S))
         H = Hkv * G
         while B * H > 1 and B * H * S * S > (1 << 31) // (2 if dtype == "float32" else 1):
             B, H, Hkv = (B - 1, H, Hkv) if B > 1 else (1, H // Hkv, 1) if Hkv > 1 else (1, 1, 1)
-        return {"op": op, "dtype": dtype, "B": B, "H": H, "Hkv": Hkv, "S": S, "D": D, "window": _log(rng, 1, 2048),
+        return {"op": op, "dtype": dtype, "B": B, "H": H, "Hkv": Hkv, "S": S, "D": D, "window": _log(rng, 4 if bwd else 1, 2048),
                 "sinks": rng.choice([0, 0, 1, 4, rng.randint(2, 130)]), "shortest": S if rng.random() < 0.5 else rng.randint(1, S)}
     Lmax = _log(rng, 64, 8192)
     B = max(1, min(_log(rng, 1, 64), (64 * 32 * 8192) // (Lmax * Hkv * 4)))
