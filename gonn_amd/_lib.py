@@ -29,7 +29,7 @@ GONN_ATTN_FP32_MFMA, GONN_ATTN_BF16_MFMA, GONN_ATTN_FP64 = 0, 1, 2
 (GONN_UN_RELU, GONN_UN_SIGMOID, GONN_UN_TANH, GONN_UN_EXP, GONN_UN_LOG, GONN_UN_GELU,
  GONN_UN_SILU, GONN_UN_GELU_EXACT) = range(8)
 GONN_BIN_ADD, GONN_BIN_SUB, GONN_BIN_MUL, GONN_BIN_DIV = range(4)
-GONN_OP_FWD, GONN_OP_BWD, GONN_OP_DECODE = 0, 1, 2
+(GONN_OP_FWD, GONN_OP_BWD, GONN_OP_DECODE, GONN_OP_WINDOW_FWD, GONN_OP_WINDOW_BWD) = range(5)
 
 # Every symbol include/gonn_hip.h declares.
 EXPORTED_SYMBOLS = (
@@ -52,6 +52,7 @@ EXPORTED_SYMBOLS = (
     "gonn_hip_attn_decode_noalloc",
     "gonn_hip_kvcache_attend_causal_workspace_bytes", "gonn_hip_kvcache_attend_causal",
     "gonn_hip_mha_incremental_workspace_bytes", "gonn_hip_mha_forward_incremental_dev",
+    "gonn_hip_attn_window_fwd", "gonn_hip_attn_window_bwd",
     "gonn_hip_calib_mfma", "gonn_hip_calib_clock_start", "gonn_hip_calib_clock_read",
 )
 
@@ -98,6 +99,23 @@ class DecodeArgs(ctypes.Structure):
                 ("D", ctypes.c_int), ("scale", ctypes.c_double), ("split_keys", ctypes.c_int)]
 
 
+class WindowFwdArgs(ctypes.Structure):
+    _fields_ = [("q", Buf), ("k", Buf), ("v", Buf), ("o", Buf), ("lse", Buf),
+                ("B", ctypes.c_int), ("H", ctypes.c_int), ("Hkv", ctypes.c_int),
+                ("Sq", ctypes.c_int), ("Sk", ctypes.c_int), ("D", ctypes.c_int),
+                ("scale", ctypes.c_double), ("window", ctypes.c_int), ("sinks", ctypes.c_int),
+                ("kv_len", Buf)]
+
+
+class WindowBwdArgs(ctypes.Structure):
+    _fields_ = [("q", Buf), ("k", Buf), ("v", Buf), ("o", Buf), ("lse", Buf), ("dO", Buf),
+                ("dq", Buf), ("dk", Buf), ("dv", Buf),
+                ("B", ctypes.c_int), ("H", ctypes.c_int), ("Hkv", ctypes.c_int),
+                ("Sq", ctypes.c_int), ("Sk", ctypes.c_int), ("D", ctypes.c_int),
+                ("scale", ctypes.c_double), ("window", ctypes.c_int), ("sinks", ctypes.c_int),
+                ("kv_len", Buf)]
+
+
 _lib = None
 
 
@@ -125,6 +143,8 @@ def load() -> ctypes.CDLL:
     lib.gonn_hip_attn_workspace_bytes.argtypes = [i, vp]
     lib.gonn_hip_attn_fwd.argtypes = [ctypes.POINTER(FwdArgs), vp, sz, vp]
     lib.gonn_hip_attn_bwd.argtypes = [ctypes.POINTER(BwdArgs), vp, sz, vp]
+    lib.gonn_hip_attn_window_fwd.argtypes = [ctypes.POINTER(WindowFwdArgs), vp, sz, vp]
+    lib.gonn_hip_attn_window_bwd.argtypes = [ctypes.POINTER(WindowBwdArgs), vp, sz, vp]
     lib.gonn_hip_attn_decode.argtypes = [ctypes.POINTER(DecodeArgs), vp, sz, vp]
     lib.gonn_hip_attn_decode_noalloc.argtypes = [ctypes.POINTER(DecodeArgs), vp]
     lib.gonn_hip_alloc.argtypes = [ctypes.POINTER(Buf), sz, i]

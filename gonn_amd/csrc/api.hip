@@ -135,6 +135,12 @@ QFold q_fold(double scale) {
     return f;
 }
 
+#define TRY_EARLY(x)                    \
+    do {                                \
+        const int _rc = (x);            \
+        if (_rc != GONN_OK) return _rc; \
+    } while (0)
+
 // ---- forward -----------------------------------------------------------
 
 int check_fwd(const gonn_attn_fwd_args* a) {
@@ -356,6 +362,78 @@ size_t bwd_ws(const gonn_attn_bwd_args* a, const DqPlan& plan) {
 }
 DqPlan bwd_dq_plan(const gonn_attn_bwd_args* a) {
     return bwd_dq_plan(bwd_mode(a), (size_t)a->B * a->H, a->S, bwd_keys_of(a), a->causal);
+}
+
+// ---- sliding-window attention ------------------------------------------
+
+bool aligned16(const gonn_buf& b) { return ((uintptr_t)b.ptr & 15) == 0; }
+
+// Checks what the two directions share and fills their common parameters.
+template <typename A>
+int check_window(const A* a, gonn::WindowParams* p) {
+    if (!a) return GONN_E_INVALID;
+    if (a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->Sq <= 0 || a->Sk <= 0 || a->D <= 0 ||
+        a->H % a->Hkv)
+        return GONN_E_INVALID;
+    if (a->window < 1 || a->sinks < 0 || !std::isfinite(a->scale)) return GONN_E_INVALID;
+    if (!head_dim_ok(a->D)) return GONN_E_UNSUPPORTED;
+    // Grids and row numbers are 32-bit.
+    if ((double)a->B * a->H * a->Sq >= 1073741824.0 || (double)a->B * a->Hkv * a->Sk >= 1073741824.0)
+        return GONN_E_UNSUPPORTED;
+    const int dt = a->q.dtype;
+    if (dt != GONN_F32 && dt != GONN_BF16) return GONN_E_INVALID;
+    const size_t nq = (size_t)a->B * a->H * a->Sq * a->D, nk = (size_t)a->B * a->Hkv * a->Sk * a->D;
+    if (!buf_ok(a->q, nq, dt) || !buf_ok(a->k, nk, dt) || !buf_ok(a->v, nk, dt) ||
+        !buf_ok(a->o, nq, dt))
+        return GONN_E_INVALID;
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o))
+        return GONN_E_INVALID;
+    if (a->lse.ptr && !buf_ok(a->lse, (size_t)a->B * a->H * a->Sq, GONN_F32)) return GONN_E_INVALID;
+    if (a->kv_len.ptr && !buf_ok(a->kv_len, (size_t)a->B, GONN_I32)) return GONN_E_INVALID;
+    *p = gonn::WindowParams{};
+    p->q = a->q.ptr;
+    p->k = a->k.ptr;
+    p->v = a->v.ptr;
+    p->B = a->B;
+    p->H = a->H;
+    p->Hkv = a->Hkv;
+    p->Sq = a->Sq;
+    p->Sk = a->Sk;
+    // Past these every key is seen, and sums with positions stay in range.
+    p->window = std::min(a->window, a->Sq);
+    p->sinks = std::min(a->sinks, a->Sk);
+    p->scale = (float)a->scale;
+    p->scale_log2 = (float)(a->scale * 1.4426950408889634);
+    p->kv_len = a->kv_len.ptr ? (const int*)a->kv_len.ptr : nullptr;
+    return GONN_OK;
+}
+
+int check_window_bwd(const gonn_attn_window_bwd_args* a, gonn::WindowParams* p) {
+    TRY_EARLY(check_window(a, p));
+    const int dt = a->q.dtype;
+    const size_t nq = (size_t)a->B * a->H * a->Sq * a->D, nk = (size_t)a->B * a->Hkv * a->Sk * a->D;
+    if (!buf_ok(a->dO, nq, dt) || !buf_ok(a->dq, nq, dt) || !buf_ok(a->dk, nk, dt) ||
+        !buf_ok(a->dv, nk, dt) || !a->lse.ptr)
+        return GONN_E_INVALID;
+    if (!aligned16(a->dO) || !aligned16(a->dq) || !aligned16(a->dk) || !aligned16(a->dv))
+        return GONN_E_INVALID;
+    p->o_in = a->o.ptr;
+    p->lse_in = (const float*)a->lse.ptr;
+    p->dO = a->dO.ptr;
+    p->dq = a->dq.ptr;
+    p->dk = a->dk.ptr;
+    p->dv = a->dv.ptr;
+    return GONN_OK;
+}
+
+// delta, then the dK/dV partials; fills p's work items and, given ws, its pointers.
+size_t window_bwd_ws(gonn::WindowParams& p, int D, int is_bf16, void* ws) {
+    const size_t delta = round_up((size_t)p.B * p.H * p.Sq * sizeof(float), 256);
+    const size_t part = gonn::plan_window_bwd(p, D, is_bf16);
+    uint8_t* w = (uint8_t*)round_up((size_t)ws, 256);
+    p.delta = (float*)w;
+    p.part = (float*)(w + delta);
+    return delta + part + 256;
 }
 
 // ---- helpers for the host shims ----------------------------------------
@@ -848,6 +926,12 @@ size_t gonn_hip_attn_workspace_bytes(int op, const void* args) {
             if (a->B <= 0 || a->H <= 0 || a->Lmax <= 0 || a->D <= 0) return 0;
             return decode_ws(a);
         }
+        case GONN_OP_WINDOW_BWD: {
+            const auto* a = (const gonn_attn_window_bwd_args*)args;
+            gonn::WindowParams p;
+            if (check_window_bwd(a, &p) != GONN_OK) return 0;
+            return window_bwd_ws(p, a->D, a->q.dtype == GONN_BF16, nullptr);
+        }
         default: return 0;
     }
 }
@@ -906,6 +990,25 @@ int gonn_hip_attn_fwd(const gonn_attn_fwd_args* a, void* ws, size_t ws_bytes, vo
     }
     ProfScope ps(mode == GONN_ATTN_BF16_MFMA ? "fwd_bf16" : "fwd_f32", s);
     return herr(gonn::launch_fwd(p, mode, a->D, a->causal, a->q.dtype == GONN_BF16, s));
+}
+
+int gonn_hip_attn_window_fwd(const gonn_attn_window_fwd_args* a, void*, size_t, void* stream) {
+    gonn::WindowParams p;
+    TRY(check_window(a, &p));
+    p.o = a->o.ptr;
+    p.lse = (float*)a->lse.ptr;
+    ProfScope ps("window_fwd", (hipStream_t)stream);
+    return herr(gonn::launch_window_fwd(p, a->D, a->q.dtype == GONN_BF16, (hipStream_t)stream));
+}
+
+int gonn_hip_attn_window_bwd(const gonn_attn_window_bwd_args* a, void* ws, size_t ws_bytes,
+                             void* stream) {
+    gonn::WindowParams p;
+    TRY(check_window_bwd(a, &p));
+    const int is_bf16 = a->q.dtype == GONN_BF16;
+    if (window_bwd_ws(p, a->D, is_bf16, ws) > ws_bytes || !ws) return GONN_E_WORKSPACE;
+    ProfScope ps("window_bwd", (hipStream_t)stream);
+    return herr(gonn::launch_window_bwd(p, a->D, is_bf16, (hipStream_t)stream));
 }
 
 int gonn_hip_attn_bwd(const gonn_attn_bwd_args* a, void* ws, size_t ws_bytes, void* stream) {

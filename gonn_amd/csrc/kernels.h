@@ -128,6 +128,36 @@ struct BwdParams {
     int kb0, nkb, dq_mode;
 };
 
+// Sliding-window attention with sinks (attn_window.hip, attn_window_bwd.hip):
+// query i sees key j when j <= i, j < kv_len[b] and (i - j < window or j <
+// sinks). q, o, dO, dq (B,H,Sq,D); k, v, dk, dv (B,Hkv,Sk,D), query head h
+// reading key head h / (H / Hkv); all of one type, bf16 or f32.
+struct WindowParams {
+    const void *q, *k, *v;
+    void* o;
+    float* lse;  // (B*H, Sq) natural log, or null (forward)
+    int B, H, Hkv, Sq, Sk;
+    int window, sinks;
+    float scale;       // signed
+    float scale_log2;  // scale * log2(e)
+    const int* kv_len;  // [B] or null (all Sk)
+    // Backward: the saved o and lse, dO, the gradients; delta (B*H, Sq) is
+    // written by the dQ kernel and read by the dK/dV kernel after it.
+    const void *o_in, *dO;
+    const float* lse_in;
+    float* delta;
+    void *dq, *dk, *dv;
+    // dK/dV work items (attn_window_bwd.hip): the (head, query stage) steps of
+    // a key block are cut in chunks of `chunk`; blocks of more than one leave
+    // partials, (B*Hkv, slots, 2, keys, D) f32, that a second kernel adds up.
+    float* part;
+    int chunk, per_block, per_sink, sink_blocks, slots;
+};
+hipError_t launch_window_fwd(const WindowParams& p, int D, int is_bf16, hipStream_t s);
+// Fills the work items of the dK/dV kernel; returns the bytes of p.part.
+size_t plan_window_bwd(WindowParams& p, int D, int is_bf16);
+hipError_t launch_window_bwd(const WindowParams& p, int D, int is_bf16, hipStream_t s);
+
 // Exact fp64 attention (attn_f64.hip): fp64 (BH, rows, d) buffers.
 struct F64Params {
     const double* q;      // (BH, Sq, d)

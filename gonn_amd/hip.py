@@ -14,6 +14,8 @@ Two layers, both over the C ABI (include/gonn_hip.h):
 2. The device-resident API on torch device tensors (torch only supplies
    device memory and the current HIP stream):
        attn_fwd, attn_bwd, attn_decode
+       attn_window_fwd, attn_window_bwd (sliding window with sinks, shared
+       key heads; new, the reference has neither)
 
 3. KVCache: a device KV cache handle for incremental decoding (new; the
    reference has none), with host fp64 and device-tensor methods.
@@ -29,8 +31,8 @@ import numpy as np
 from . import _lib
 from ._lib import (GONN_ATTN_BF16_MFMA, GONN_ATTN_FP32_MFMA, GONN_ATTN_FP64, GONN_BF16,
                    GONN_F32, GONN_I32,
-                   GONN_OP_BWD, GONN_OP_DECODE, GONN_OP_FWD, Buf, BwdArgs, DecodeArgs, FwdArgs,
-                   GonnHipError, check)
+                   GONN_OP_BWD, GONN_OP_DECODE, GONN_OP_FWD, GONN_OP_WINDOW_BWD, Buf, BwdArgs,
+                   DecodeArgs, FwdArgs, GonnHipError, WindowBwdArgs, WindowFwdArgs, check)
 
 MODES = {"fp32": GONN_ATTN_FP32_MFMA, "bf16": GONN_ATTN_BF16_MFMA,
          GONN_ATTN_FP32_MFMA: GONN_ATTN_FP32_MFMA, GONN_ATTN_BF16_MFMA: GONN_ATTN_BF16_MFMA}
@@ -472,6 +474,122 @@ def attn_decode(q, kcache, vcache, kv_len, *, scale=None, split_keys: int = 0, o
     return out
 
 
+class _OnStream:
+    """The device of `t` and the stream of a call, with the call's allocations on
+    that stream; tensors used on a stream other than the current one are marked
+    as used there, so that torch does not reuse their memory too early."""
+
+    def __init__(self, t, stream, tensors):
+        torch = _torch()
+        live = [x for x in tensors if x is not None]
+        for x in live:
+            if x.device != t.device:
+                raise ValueError(f"tensors on {x.device} and {t.device}")
+        self._dev = torch.cuda.device(t.device)
+        current = torch.cuda.current_stream(t.device)
+        self.stream = current if stream is None else stream
+        self._use = torch.cuda.stream(self.stream)
+        if self.stream.cuda_stream != current.cuda_stream:
+            for x in live:
+                x.record_stream(self.stream)
+
+    def __enter__(self):
+        self._dev.__enter__()
+        self._use.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        self._use.__exit__(*exc)
+        self._dev.__exit__(*exc)
+
+    @property
+    def ptr(self):
+        return ctypes.c_void_p(self.stream.cuda_stream)
+
+    def workspace(self, nbytes, device):
+        """Workspace of one call. Inside a graph capture each call has its own,
+        from the graph's pool: the shared one may grow (and move) later, and two
+        graphs that share it could not run side by side."""
+        torch = _torch()
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+        return _WS.get(nbytes, device, self.stream)
+
+
+def _window_shapes(what, q, k, v):
+    B, H, Sq, D = _shape4(q, "q")
+    Bk, Hkv, Sk, Dk = _shape4(k, "k")
+    if tuple(v.shape) != tuple(k.shape):
+        raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    if Bk != B or Dk != D or Hkv == 0 or H % Hkv:
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit together")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{what}: q, k and v must have one dtype")
+    return B, H, Hkv, Sq, Sk, D
+
+
+def _window_like(what, name, t, ref):
+    if tuple(t.shape) != tuple(ref.shape) or t.dtype != ref.dtype:
+        raise ValueError(f"{what}: {name} must be {tuple(ref.shape)} {ref.dtype}, got "
+                         f"{tuple(t.shape)} {t.dtype}")
+
+
+def attn_window_fwd(q, k, v, *, window: int, sinks: int = 0, scale=None, kv_len=None, out=None,
+                    lse=True, lse_out=None, stream=None):
+    """Causal attention over a sliding window with sinks on device tensors: query i
+    sees key j when j <= i, j < kv_len and (i - j < window or j < sinks).
+
+    q (B,H,Sq,D); k, v (B,Hkv,Sk,D) with H a multiple of Hkv (query head h reads
+    key head h // (H // Hkv)), or 3-D with one head. All float32 (fp32 accuracy) or
+    all bfloat16. Returns (O, LSE): O like q, LSE float32 (B*H, Sq) in natural-log
+    units (None when lse is False); a query that sees no key has O = 0, LSE = -inf.
+    kv_len: optional int32 device tensor (B,). New relative to the reference."""
+    torch = _torch()
+    B, H, Hkv, Sq, Sk, D = _window_shapes("attn_window_fwd", q, k, v)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    with _OnStream(q, stream, (q, k, v, kv_len, out, lse_out)) as on:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _window_like("attn_window_fwd", "out", out, q)
+        if lse_out is None and lse:
+            lse_out = torch.empty((B * H, Sq), dtype=torch.float32, device=q.device)
+        a = WindowFwdArgs(buf(q), buf(k), buf(v), buf(out), buf(lse_out), B, H, Hkv, Sq, Sk, D,
+                          float(scale), int(window), int(sinks), buf(kv_len))
+        check(_lib.load().gonn_hip_attn_window_fwd(ctypes.byref(a), None, 0, on.ptr),
+              "attn_window_fwd")
+    return out, lse_out
+
+
+def attn_window_bwd(q, k, v, o, lse, dO, *, window: int, sinks: int = 0, scale=None, kv_len=None,
+                    out=None, stream=None):
+    """dQ, dK, dV of attn_window_fwd from its saved o and lse, in the inputs' dtype;
+    dK and dV of a key head are summed over the query heads that read it. out may
+    supply preallocated (dq, dk, dv). Deterministic."""
+    torch = _torch()
+    what = "attn_window_bwd"
+    B, H, Hkv, Sq, Sk, D = _window_shapes(what, q, k, v)
+    _window_like(what, "o", o, q)
+    _window_like(what, "dO", dO, q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    given = out if out is not None else ()
+    with _OnStream(q, stream, (q, k, v, o, lse, dO, kv_len, *given)) as on:
+        dq, dk, dv = out if out is not None else (torch.empty_like(x) for x in (q, k, v))
+        for name, t, ref in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+            _window_like(what, name, t, ref)
+        a = WindowBwdArgs(buf(q), buf(k), buf(v), buf(o), buf(lse), buf(dO), buf(dq), buf(dk),
+                          buf(dv), B, H, Hkv, Sq, Sk, D, float(scale), int(window), int(sinks),
+                          buf(kv_len))
+        lib = _lib.load()
+        nb = lib.gonn_hip_attn_workspace_bytes(GONN_OP_WINDOW_BWD, ctypes.byref(a))
+        ws = on.workspace(nb, q.device)
+        check(lib.gonn_hip_attn_window_bwd(ctypes.byref(a),
+                                           ws.data_ptr() if ws is not None else None, nb, on.ptr),
+              what)
+    return dq, dk, dv
+
+
 # ---------------------------------------------------------------------------
 # KV cache (incremental decoding)
 # ---------------------------------------------------------------------------
@@ -744,4 +862,4 @@ __all__ = ["Available", "Supports", "SetAttnMode", "AttnMode", "Version", "Selft
            "FlashAttnF64BwdEx", "mask_strides", "Gemm",
            "Unary", "Binary",
            "BenchFlashAttnF64", "BenchFlashAttnF64Bwd", "attn_fwd", "attn_bwd", "attn_decode",
-           "KVCache", "DeviceMHA", "buf", "GonnHipError"]
+           "attn_window_fwd", "attn_window_bwd", "KVCache", "DeviceMHA", "buf", "GonnHipError"]

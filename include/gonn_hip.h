@@ -160,7 +160,48 @@ typedef struct {
     int split_keys;
 } gonn_attn_decode_args;
 
-enum { GONN_OP_FWD = 0, GONN_OP_BWD = 1, GONN_OP_DECODE = 2 };
+/* Sliding-window attention with sinks (no counterpart in the reference, whose
+ * masks are the causal one, key padding and an additive array): query i sees
+ * key j when j <= i, j < kv_len[b] and (i - j < window or j < sinks).
+ *   s_ij = scale q_i . k_j,  LSE_i = ln sum_j exp(s_ij),  O_i = sum_j exp(s_ij - LSE_i) v_j
+ * over the keys that i sees; a query that sees none gets O = 0, LSE = -inf.
+ * q, o (B,H,Sq,D); k, v (B,Hkv,Sk,D) with H a multiple of Hkv: query head h
+ * reads key head h / (H / Hkv). All of one type, GONN_F32 (fp32 accuracy) or
+ * GONN_BF16 (bf16 products and weights, fp32 sums); lse (B*H,Sq) GONN_F32 or
+ * ptr NULL. Buffers 16-byte aligned. window >= 1 (Sq or more: no window),
+ * sinks >= 0; kv_len: GONN_I32 device array [B] or ptr NULL, clamped to
+ * [0, Sk]. An infinity or a NaN in a key or value reaches only the queries that
+ * see that key.                                                            */
+typedef struct {
+    gonn_buf q, k, v, o, lse;
+    int B, H, Hkv, Sq, Sk, D;
+    double scale;
+    int window, sinks;
+    gonn_buf kv_len;
+} gonn_attn_window_fwd_args;
+
+/* Its backward from the saved o and lse:
+ *   P_ij = exp(s_ij - LSE_i), dV_j = sum_i P_ij dO_i,
+ *   dS_ij = P_ij (dO_i . v_j - dO_i . O_i),
+ *   dQ_i = scale sum_j dS_ij k_j, dK_j = scale sum_i dS_ij q_i,
+ * dK and dV of a key head summed over its H / Hkv query heads. dO, dq like q;
+ * dk, dv like k; the other arguments as in the forward. Keys at and past
+ * kv_len get dK = dV = 0, a query without keys dQ = 0. Deterministic.      */
+typedef struct {
+    gonn_buf q, k, v, o, lse, dO, dq, dk, dv;
+    int B, H, Hkv, Sq, Sk, D;
+    double scale;
+    int window, sinks;
+    gonn_buf kv_len;
+} gonn_attn_window_bwd_args;
+
+enum {
+    GONN_OP_FWD = 0,
+    GONN_OP_BWD = 1,
+    GONN_OP_DECODE = 2,
+    GONN_OP_WINDOW_FWD = 3,
+    GONN_OP_WINDOW_BWD = 4
+};
 
 /* ---- library ----------------------------------------------------------- */
 
@@ -193,7 +234,7 @@ int gonn_hip_get_attn_mode(void);
 /* ---- device-resident API ---------------------------------------------- */
 
 /* Workspace bytes a call with these arguments needs (0 if none).
- * op: GONN_OP_FWD / GONN_OP_BWD / GONN_OP_DECODE with the matching struct. */
+ * op: GONN_OP_* with the matching struct.                                  */
 size_t gonn_hip_attn_workspace_bytes(int op, const void* args);
 
 /* Flash forward. Replaces gonn_flash_attn_f64_fwd
@@ -210,6 +251,15 @@ int gonn_hip_attn_fwd(const gonn_attn_fwd_args* a, void* ws, size_t ws_bytes, vo
  * workspace query alike: GONN_HIP_BWD_DS_MB=<MB> sets the dS budget and always
  * chunks within it; GONN_HIP_BWD_DQ=recompute forms dS again.               */
 int gonn_hip_attn_bwd(const gonn_attn_bwd_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/* Sliding-window attention with sinks, forward and backward (see the argument
+ * structs). ws: gonn_hip_attn_workspace_bytes(GONN_OP_WINDOW_FWD / _BWD) bytes
+ * (the forward needs none); calls that share one must not overlap. Only kernel
+ * launches on `stream`: both can be captured in a HIP graph.               */
+int gonn_hip_attn_window_fwd(const gonn_attn_window_fwd_args* a, void* ws, size_t ws_bytes,
+                             void* stream);
+int gonn_hip_attn_window_bwd(const gonn_attn_window_bwd_args* a, void* ws, size_t ws_bytes,
+                             void* stream);
 
 /* Split-KV decode plus combine. New: the reference has no KV cache; the
  * semantics are ForwardMasked with WithKeyPaddingMask (nn/attention.go:305-341,
