@@ -122,6 +122,7 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
         f32x16 s = f32x16{};
         for (int k = 0; k < NKS; k++) s = mfma_n(tile_row<D, NP>(tl, tile, 0, k), qf[k], s);
         s *= c2;
+        pin_before_branch(s);
         if (kb + 32 > kl || !band.all(qw, qw + 31, kb, kb + 31))
             for (int r = 0; r < 16; r++) {
                 const int key = kb + 8 * (r >> 2) + 4 * g + (r & 3);

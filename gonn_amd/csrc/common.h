@@ -318,6 +318,16 @@ GONN_DEV void pin(const T& x) {
     asm volatile("" ::"v"(x));
 }
 
+// pin on a value formed from MFMA results, ahead of a branch. The compiler may sink
+// such VALU work below the branch, and the wait states that it inserts there have
+// been too few on the taken path (an accumulator's last registers were read 2 to 7
+// states after a 32x32x16 MFMA, which needs 11): pinned, the work stays behind the
+// MFMA in its own block, where they are right.
+template <typename T>
+GONN_DEV void pin_before_branch(const T& x) {
+    pin(x);
+}
+
 // Compile-time loop: f(std::integral_constant<int, i>) for i = 0 .. N-1.
 template <typename F, int... I>
 GONN_DEV void static_for_impl(F&& f, std::integer_sequence<int, I...>) {
