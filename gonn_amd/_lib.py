@@ -53,6 +53,9 @@ EXPORTED_SYMBOLS = (
     "gonn_hip_kvcache_attend_causal_workspace_bytes", "gonn_hip_kvcache_attend_causal",
     "gonn_hip_mha_incremental_workspace_bytes", "gonn_hip_mha_forward_incremental_dev",
     "gonn_hip_attn_window_fwd", "gonn_hip_attn_window_bwd",
+    "gonn_hip_kvcache8_create", "gonn_hip_kvcache8_free", "gonn_hip_kvcache8_lengths",
+    "gonn_hip_kvcache8_append", "gonn_hip_kvcache8_truncate", "gonn_hip_kvcache8_read",
+    "gonn_hip_kvcache8_attend_workspace_bytes", "gonn_hip_kvcache8_attend",
     "gonn_hip_calib_mfma", "gonn_hip_calib_clock_start", "gonn_hip_calib_clock_read",
 )
 
@@ -208,6 +211,16 @@ def load() -> ctypes.CDLL:
     lib.gonn_hip_mha_incremental_workspace_bytes.argtypes = [vp, vp, i]
     lib.gonn_hip_mha_forward_incremental_dev.argtypes = [vp, vp, ctypes.POINTER(Buf),
                                                          ctypes.POINTER(Buf), i, vp, sz, vp]
+    bp = ctypes.POINTER(Buf)
+    lib.gonn_hip_kvcache8_create.argtypes = [ctypes.POINTER(vp), i, i, i, i]
+    lib.gonn_hip_kvcache8_free.argtypes = [vp]
+    lib.gonn_hip_kvcache8_lengths.argtypes = [vp, ip, vp]
+    lib.gonn_hip_kvcache8_append.argtypes = [vp, bp, bp, i, ip, vp]
+    lib.gonn_hip_kvcache8_truncate.argtypes = [vp, ip, vp]
+    lib.gonn_hip_kvcache8_read.argtypes = [vp, bp, bp, i, i, vp]
+    lib.gonn_hip_kvcache8_attend_workspace_bytes.restype = sz
+    lib.gonn_hip_kvcache8_attend_workspace_bytes.argtypes = [vp, i, i, i, i, vp]
+    lib.gonn_hip_kvcache8_attend.argtypes = [vp, bp, bp, i, i, ctypes.c_double, i, i, vp, sz, vp]
     _lib = lib
     return lib
 

@@ -20,6 +20,7 @@
 #include "common.h"
 #include "host_xfer.h"
 #include "kernels.h"
+#include "kvcache8.h"
 #include "kvcache_internal.h"
 
 #define GONN_HIP_VERSION "gonn-hip 0.1.0 (gfx950)"
@@ -779,6 +780,97 @@ AttendPlan attend_plan(const gonn_kvcache* c, int T) {
     }
     q.nsplit = (c->Lmax + q.split_keys - 1) / q.split_keys;
     return q;
+}
+
+}  // namespace
+
+// The 8-bit cache's handle. The lengths on the device are the ones that count;
+// the host follows them as long as it knows every call that changes them.
+struct gonn_kvcache8 {
+    gonn::Cache8 c{};
+    void* mem = nullptr;  // everything on the device
+    std::vector<int> len, lo;
+    // A call that changes the lengths was captured in a graph: they may advance
+    // without the host, which reads them back where it needs them.
+    bool captured = false;
+};
+
+namespace {
+
+bool stream_captures(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return st == hipStreamCaptureStatusActive;
+}
+
+// The device's lengths on the host (waits for s) if the host may not know them.
+int cache8_refresh(gonn_kvcache8* h, hipStream_t s) {
+    if (!h->captured) return GONN_OK;
+    const size_t n = (size_t)h->c.B * sizeof(int);
+    TRYH(hipMemcpyAsync(h->len.data(), h->c.len, n, hipMemcpyDeviceToHost, s));
+    TRYH(hipMemcpyAsync(h->lo.data(), h->c.lo, n, hipMemcpyDeviceToHost, s));
+    return herr(hipStreamSynchronize(s));
+}
+
+// f(Seqs8) for every kSeqs8 sequences; n: per-sequence numbers, or null for `all`.
+template <typename F>
+int each_seqs8(int B, const int* n, int all, F f) {
+    for (int b0 = 0; b0 < B; b0 += gonn::kSeqs8) {
+        gonn::Seqs8 q;
+        q.b0 = b0;
+        q.nb = std::min(B - b0, gonn::kSeqs8);
+        q.use = n != nullptr;
+        q.all = all;
+        for (int i = 0; i < gonn::kSeqs8; i++) q.n[i] = n && i < q.nb ? n[b0 + i] : 0;
+        TRYH(f(q));
+    }
+    return GONN_OK;
+}
+
+// Rows per workgroup, blocks per split and splits of an attend. Whole rows of 32
+// go to key waves while one wave holds them all.
+struct Plan8 {
+    int rows, split, nsplit;
+};
+Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks, hipStream_t s) {
+    const gonn::Cache8& c = h->c;
+    const long long R = (long long)Hq / c.H * T, cus = gonn::device_cus();
+    Plan8 p{};
+    p.rows = R <= 32 ? 32 : (R <= 64 ? 64 : 128);
+    int longest = c.Lmax;
+    if (!h->captured && !stream_captures(s)) longest = *std::max_element(h->len.begin(), h->len.end());
+    long long blocks = (longest + gonn::kBlk8 - 1) / gonn::kBlk8;
+    if (window > 0) {
+        const long long seen = ((long long)window + T + 2 * gonn::kBlk8 - 3) / gonn::kBlk8 +
+                               ((long long)sinks + gonn::kBlk8 - 1) / gonn::kBlk8;
+        blocks = std::min(blocks, seen);
+    }
+    blocks = std::max<long long>(blocks, 1);
+    const long long units = (long long)c.B * c.H * ((R + p.rows - 1) / p.rows);
+    // Splits of 32 blocks level out sequences of different lengths; shorter ones
+    // where the device has room for more workgroups, down to a block per key wave.
+    const long long want = 4 * cus, least = 128 / p.rows;
+    long long split = 32;
+    if (units * ((blocks + split - 1) / split) < want)
+        split = std::max(least, blocks * units / want);
+    p.split = (int)std::max<long long>(1, split);
+    p.nsplit = (int)((blocks + p.split - 1) / p.split);
+    return p;
+}
+
+size_t attend8_ws(const gonn_kvcache8* h, int Hq, int T, const Plan8& p) {
+    if (p.nsplit <= 1) return 0;
+    const size_t parts = (size_t)h->c.B * Hq * T * p.nsplit;
+    return round_up(parts * 2, 64) * sizeof(float) + parts * h->c.D * sizeof(float) + 512;
+}
+
+int check_attend8(const gonn_kvcache8* h, int Hq, int T, int window, int sinks) {
+    if (!h || Hq <= 0 || T <= 0 || Hq % h->c.H || window < 0 || sinks < 0) return GONN_E_INVALID;
+    if ((double)h->c.B * Hq * T >= 1073741824.0) return GONN_E_UNSUPPORTED;
+    return GONN_OK;
 }
 
 }  // namespace
@@ -1898,6 +1990,187 @@ int gonn_hip_kvcache_attend_causal(gonn_kvcache* c, const gonn_buf* q, gonn_buf*
     if (!ws || ws_bytes < gonn::kvcache_attend_causal_ws(c, T)) return GONN_E_WORKSPACE;
     return gonn::kvcache_attend_causal_run(c, (const float*)q->ptr, (float*)o->ptr, T, scale, ws,
                                            (hipStream_t)stream, true);
+}
+
+// ---- KV cache in 8 bits ------------------------------------------------------
+
+int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D) {
+    if (!out) return GONN_E_INVALID;
+    *out = nullptr;
+    if (B <= 0 || H <= 0 || Lmax <= 0 || D <= 0) return GONN_E_INVALID;
+    if (!head_dim_ok(D)) return GONN_E_UNSUPPORTED;
+    if ((double)B * H * ((double)Lmax + 128) >= 1073741824.0) return GONN_E_UNSUPPORTED;
+    if (!gonn_hip_available()) return GONN_E_NODEVICE;
+    if (fail_alloc_injected()) return GONN_E_INJECTED;
+    gonn_kvcache8* h = nullptr;
+    try {
+        h = new gonn_kvcache8;
+        h->len.assign(B, 0);
+        h->lo.assign(B, 0);
+    } catch (const std::bad_alloc&) {
+        delete h;
+        return GONN_E_NOMEM;
+    }
+    gonn::Cache8& c = h->c;
+    c.B = B;
+    c.H = H;
+    c.Lmax = Lmax;
+    c.D = D;
+    c.nblk = std::max(1, Lmax / gonn::kBlk8);
+    const size_t BH = (size_t)B * H, codes = BH * c.nblk * gonn::kBlk8 * D,
+                 ring = BH * 2 * gonn::kBlk8 * D * sizeof(uint16_t),
+                 scales = round_up(BH * c.nblk * sizeof(float), 256),
+                 lens = round_up((size_t)B * sizeof(int), 256);
+    const size_t bytes = 2 * codes + 2 * scales + 2 * ring + 2 * lens + 256;
+    if (hipMalloc(&h->mem, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        delete h;
+        return GONN_E_NOMEM;
+    }
+    uint8_t* p = (uint8_t*)h->mem;
+    auto take = [&p](size_t n) {
+        uint8_t* r = p;
+        p += n;
+        return r;
+    };
+    c.k8 = take(codes);
+    c.v8 = take(codes);
+    c.ks = (float*)take(scales);
+    c.vs = (float*)take(scales);
+    c.kt = (uint16_t*)take(ring);
+    c.vt = (uint16_t*)take(ring);
+    uint8_t* state = p;
+    c.len = (int*)take(lens);
+    c.lo = (int*)take(lens);
+    c.ticket = (unsigned*)take(256);
+    hipError_t e = hipMemset(state, 0, 2 * lens + 256);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        (void)hipFree(h->mem);
+        delete h;
+        return herr(e);
+    }
+    *out = h;
+    return GONN_OK;
+}
+
+int gonn_hip_kvcache8_free(gonn_kvcache8* h) {
+    if (!h) return GONN_OK;
+    (void)hipFree(h->mem);
+    delete h;
+    return GONN_OK;
+}
+
+int gonn_hip_kvcache8_lengths(gonn_kvcache8* h, int* len, void* stream) {
+    if (!h || !len) return GONN_E_INVALID;
+    TRY(cache8_refresh(h, (hipStream_t)stream));
+    std::copy(h->len.begin(), h->len.end(), len);
+    return GONN_OK;
+}
+
+int gonn_hip_kvcache8_append(gonn_kvcache8* h, const gonn_buf* k, const gonn_buf* v, int T,
+                             const int* counts, void* stream) {
+    if (!h || !k || !v || T <= 0) return GONN_E_INVALID;
+    const gonn::Cache8& c = h->c;
+    if (k->dtype != v->dtype || (k->dtype != GONN_F32 && k->dtype != GONN_BF16)) return GONN_E_INVALID;
+    const size_t n = (size_t)c.B * c.H * T * c.D;
+    if (!buf_ok(*k, n, k->dtype) || !buf_ok(*v, n, v->dtype) || !aligned16(*k) || !aligned16(*v))
+        return GONN_E_INVALID;
+    if ((double)c.B * c.H * ((double)T + 128) / 64 >= 2147483647.0) return GONN_E_UNSUPPORTED;
+    hipStream_t s = (hipStream_t)stream;
+    const bool capturing = stream_captures(s);
+    if (!capturing) TRY(cache8_refresh(h, s));
+    for (int b = 0; b < c.B; b++) {
+        const int m = counts ? counts[b] : T;
+        if (m < 0 || m > T || (long long)h->len[b] + m > c.Lmax) return GONN_E_INVALID;
+    }
+    {
+        ProfScope ps("kv8_append", s);
+        TRY(each_seqs8(c.B, counts, T, [&](const gonn::Seqs8& q) {
+            return gonn::launch_append8(c, k->ptr, v->ptr, k->dtype == GONN_BF16, T, q, s);
+        }));
+    }
+    if (capturing) {
+        h->captured = true;
+        return GONN_OK;
+    }
+    for (int b = 0; b < c.B; b++) {
+        h->len[b] += counts ? counts[b] : T;
+        h->lo[b] = std::max(h->lo[b], (h->len[b] / gonn::kBlk8 - 1) * gonn::kBlk8);
+    }
+    return GONN_OK;
+}
+
+int gonn_hip_kvcache8_truncate(gonn_kvcache8* h, const int* len, void* stream) {
+    if (!h || !len) return GONN_E_INVALID;
+    const gonn::Cache8& c = h->c;
+    hipStream_t s = (hipStream_t)stream;
+    const bool capturing = stream_captures(s);
+    if (!capturing) TRY(cache8_refresh(h, s));
+    for (int b = 0; b < c.B; b++) {
+        if (len[b] < 0 || len[b] > (capturing ? c.Lmax : h->len[b])) return GONN_E_INVALID;
+        if (!capturing && len[b] < h->lo[b] && len[b] % gonn::kBlk8) return GONN_E_UNSUPPORTED;
+    }
+    TRY(each_seqs8(c.B, len, 0, [&](const gonn::Seqs8& q) { return gonn::launch_truncate8(c, q, s); }));
+    if (capturing) {
+        h->captured = true;
+        return GONN_OK;
+    }
+    for (int b = 0; b < c.B; b++) {
+        h->len[b] = len[b];
+        h->lo[b] = std::min(h->lo[b], len[b] / gonn::kBlk8 * gonn::kBlk8);
+    }
+    return GONN_OK;
+}
+
+int gonn_hip_kvcache8_read(gonn_kvcache8* h, gonn_buf* k, gonn_buf* v, int start, int count,
+                           void* stream) {
+    if (!h || !k || !v || start < -1 || count <= 0 || count > h->c.Lmax || start > h->c.Lmax)
+        return GONN_E_INVALID;
+    const gonn::Cache8& c = h->c;
+    const size_t n = (size_t)c.B * c.H * count * c.D;
+    if (!buf_ok(*k, n, GONN_BF16) || !buf_ok(*v, n, GONN_BF16) || !aligned16(*k) || !aligned16(*v))
+        return GONN_E_INVALID;
+    return herr(gonn::launch_read8(c, k->ptr, v->ptr, start, count, (hipStream_t)stream));
+}
+
+size_t gonn_hip_kvcache8_attend_workspace_bytes(const gonn_kvcache8* h, int Hq, int T, int window,
+                                                int sinks, void* stream) {
+    if (check_attend8(h, Hq, T, window, sinks) != GONN_OK) return 0;
+    return attend8_ws(h, Hq, T, attend8_plan(h, Hq, T, window, sinks, (hipStream_t)stream));
+}
+
+int gonn_hip_kvcache8_attend(gonn_kvcache8* h, const gonn_buf* q, gonn_buf* o, int Hq, int T,
+                             double scale, int window, int sinks, void* ws, size_t ws_bytes,
+                             void* stream) {
+    TRY(check_attend8(h, Hq, T, window, sinks));
+    if (!q || !o || !std::isfinite(scale) || q->dtype != o->dtype ||
+        (q->dtype != GONN_F32 && q->dtype != GONN_BF16))
+        return GONN_E_INVALID;
+    const size_t n = (size_t)h->c.B * Hq * T * h->c.D;
+    if (!buf_ok(*q, n, q->dtype) || !buf_ok(*o, n, o->dtype) || !aligned16(*q) || !aligned16(*o))
+        return GONN_E_INVALID;
+    hipStream_t s = (hipStream_t)stream;
+    const Plan8 plan = attend8_plan(h, Hq, T, window, sinks, s);
+    const size_t need = attend8_ws(h, Hq, T, plan);
+    if (need && (!ws || ws_bytes < need)) return GONN_E_WORKSPACE;
+    gonn::Attend8 a{};
+    a.c = h->c;
+    a.q = q->ptr;
+    a.o = o->ptr;
+    a.Hq = Hq;
+    a.T = T;
+    a.window = window;
+    a.sinks = window ? sinks : 0;
+    a.rows = plan.rows;
+    a.split = plan.split;
+    a.nsplit = plan.nsplit;
+    a.scale_log2 = (float)(scale * 1.4426950408889634);
+    float* w = (float*)round_up((size_t)ws, 256);
+    a.part_ml = w;
+    a.part_o = w + round_up((size_t)h->c.B * Hq * T * plan.nsplit * 2, 64);
+    ProfScope ps("kv8_attend", s);
+    return herr(gonn::launch_attend8(a, q->dtype == GONN_BF16, s));
 }
 
 }  // extern "C"

@@ -18,7 +18,9 @@ Two layers, both over the C ABI (include/gonn_hip.h):
        key heads; new, the reference has neither)
 
 3. KVCache: a device KV cache handle for incremental decoding (new; the
-   reference has none), with host fp64 and device-tensor methods.
+   reference has none), with host fp64 and device-tensor methods. KVCache8: the
+   same in 8 bits, with shared key heads, a sliding window and sinks, on device
+   tensors and without host synchronisation.
 """
 from __future__ import annotations
 
@@ -475,36 +477,40 @@ def attn_decode(q, kcache, vcache, kv_len, *, scale=None, split_keys: int = 0, o
 
 
 class _OnStream:
-    """The device of `t` and the stream of a call, with the call's allocations on
-    that stream; tensors used on a stream other than the current one are marked
-    as used there, so that torch does not reuse their memory too early."""
+    """A call's device and stream, with the call's allocations on that stream;
+    tensors used on a stream other than the current one are marked as used there,
+    so that torch does not reuse their memory too early. The usual call, on the
+    current device and stream, switches neither."""
 
-    def __init__(self, t, stream, tensors):
+    def __init__(self, device, stream, tensors):
         torch = _torch()
-        live = [x for x in tensors if x is not None]
-        for x in live:
-            if x.device != t.device:
-                raise ValueError(f"tensors on {x.device} and {t.device}")
-        self._dev = torch.cuda.device(t.device)
-        current = torch.cuda.current_stream(t.device)
+        for x in tensors:
+            if x is not None and x.device != device:
+                raise ValueError(f"tensors on {x.device} and {device}")
+        if device.type != "cuda":
+            raise ValueError(f"device API needs device tensors, not {device.type} ones")
+        current = torch.cuda.current_stream(device)
         self.stream = current if stream is None else stream
-        self._use = torch.cuda.stream(self.stream)
+        self._enter = []
+        if device.index is not None and device.index != torch.cuda.current_device():
+            self._enter.append(torch.cuda.device(device))
         if self.stream.cuda_stream != current.cuda_stream:
-            for x in live:
-                x.record_stream(self.stream)
+            self._enter.append(torch.cuda.stream(self.stream))
+            for x in tensors:
+                if x is not None:
+                    x.record_stream(self.stream)
+        elif self._enter:
+            self._enter.append(torch.cuda.stream(self.stream))
+        self.ptr = ctypes.c_void_p(self.stream.cuda_stream)
 
     def __enter__(self):
-        self._dev.__enter__()
-        self._use.__enter__()
+        for c in self._enter:
+            c.__enter__()
         return self
 
     def __exit__(self, *exc):
-        self._use.__exit__(*exc)
-        self._dev.__exit__(*exc)
-
-    @property
-    def ptr(self):
-        return ctypes.c_void_p(self.stream.cuda_stream)
+        for c in reversed(self._enter):
+            c.__exit__(*exc)
 
     def workspace(self, nbytes, device):
         """Workspace of one call. Inside a graph capture each call has its own,
@@ -548,7 +554,7 @@ def attn_window_fwd(q, k, v, *, window: int, sinks: int = 0, scale=None, kv_len=
     B, H, Hkv, Sq, Sk, D = _window_shapes("attn_window_fwd", q, k, v)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _OnStream(q, stream, (q, k, v, kv_len, out, lse_out)) as on:
+    with _OnStream(q.device, stream, (q, k, v, kv_len, out, lse_out)) as on:
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _window_like("attn_window_fwd", "out", out, q)
@@ -574,7 +580,7 @@ def attn_window_bwd(q, k, v, o, lse, dO, *, window: int, sinks: int = 0, scale=N
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     given = out if out is not None else ()
-    with _OnStream(q, stream, (q, k, v, o, lse, dO, kv_len, *given)) as on:
+    with _OnStream(q.device, stream, (q, k, v, o, lse, dO, kv_len, *given)) as on:
         dq, dk, dv = out if out is not None else (torch.empty_like(x) for x in (q, k, v))
         for name, t, ref in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
             _window_like(what, name, t, ref)
@@ -723,6 +729,140 @@ class KVCache:
         return out
 
 
+class KVCache8:
+    """A device KV cache in 8 bits (gonn_hip_kvcache8_*): K and V of B sequences x H
+    key heads, up to Lmax positions of head dim D (64 or 128). Complete blocks of 64
+    positions are held in e4m3 with a power-of-two scale per block, head and tensor,
+    the last, incomplete block in bfloat16; what it holds is a function of the
+    sequence alone, however that was appended. New relative to the reference.
+
+    Calls run on torch's current stream (or `stream`) and do not wait for it; they
+    can be captured in a graph, after which lengths() and truncate() read the
+    lengths back from the device."""
+
+    BLOCK = 64
+
+    def __init__(self, B: int, H: int, Lmax: int, D: int):
+        self.B, self.H, self.Lmax, self.D = int(B), int(H), int(Lmax), int(D)
+        self._h = ctypes.c_void_p()
+        check(_lib.load().gonn_hip_kvcache8_create(ctypes.byref(self._h), self.B, self.H,
+                                                   self.Lmax, self.D), "KVCache8")
+        self.device = _torch().device("cuda", _torch().cuda.current_device())
+
+    def close(self) -> None:
+        if self._h:
+            check(_lib.load().gonn_hip_kvcache8_free(self._h), "KVCache8.close")
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def _live(self):
+        if not self._h:
+            raise ValueError("KVCache8: closed")
+        return self._h
+
+    def _on(self, stream, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"KVCache8: a tensor on {t.device}, the cache on {self.device}")
+        return _OnStream(self.device, stream, tensors)
+
+    def _ints(self, n, what):
+        a = np.ascontiguousarray(n, dtype=np.int32)
+        if a.shape != (self.B,):
+            raise ValueError(f"KVCache8: {what} must have {self.B} entries")
+        return a, a.ctypes.data_as(ctypes.POINTER(ctypes.c_int))
+
+    def lengths(self, stream=None) -> np.ndarray:
+        out, p = self._ints(np.zeros(self.B), "lengths")
+        with self._on(stream) as on:
+            check(_lib.load().gonn_hip_kvcache8_lengths(self._live(), p, on.ptr), "KVCache8.lengths")
+        return out
+
+    def append(self, k, v, counts=None, stream=None) -> None:
+        """k, v device (B,H,T,D) float32 or bfloat16 (both the same); sequence b takes
+        its first counts[b] rows (host numbers; all T when None)."""
+        if k.dim() != 4 or tuple(k.shape) != tuple(v.shape) or k.shape[0] != self.B \
+                or k.shape[1] != self.H or k.shape[3] != self.D:
+            raise ValueError(f"KVCache8.append: k, v must be ({self.B},{self.H},T,{self.D})")
+        c, cp = (None, None) if counts is None else self._ints(counts, "counts")
+        with self._on(stream, k, v) as on:
+            check(_lib.load().gonn_hip_kvcache8_append(
+                self._live(), ctypes.byref(buf(k)), ctypes.byref(buf(v)), int(k.shape[2]), cp,
+                on.ptr), "KVCache8.append")
+
+    def truncate(self, lengths, stream=None) -> None:
+        """Drops the positions from lengths[b] on (host numbers). Any multiple of 64, or
+        back to the start of the block before the one that the longest append so far
+        ended in; the cache is then what it was at that length."""
+        n, p = self._ints(lengths, "lengths")
+        with self._on(stream) as on:
+            check(_lib.load().gonn_hip_kvcache8_truncate(self._live(), p, on.ptr),
+                  "KVCache8.truncate")
+
+    def reset(self, stream=None) -> None:
+        """Drops every position."""
+        self.truncate(np.zeros(self.B), stream)
+
+    def read(self, start=None, count=None, *, last=None, out=None, stream=None):
+        """(k, v) bfloat16 (B,H,count,D): the numbers that positions start .. start +
+        count - 1 are held as (or, with last=n, each sequence's last n), zeros where a
+        sequence has none. out may supply the two tensors."""
+        torch = _torch()
+        if (last is None) == (start is None) or (start is not None and (count is None or start < 0)):
+            raise ValueError("KVCache8.read: give start and count, or last")
+        n = int(last if last is not None else count)
+        shape = (self.B, self.H, n, self.D)
+        with self._on(stream, *(out or ())) as on:
+            k, v = out if out is not None else (
+                torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+            for t in (k, v):
+                if tuple(t.shape) != shape:
+                    raise ValueError(f"KVCache8.read: out must be {shape}")
+            check(_lib.load().gonn_hip_kvcache8_read(
+                self._live(), ctypes.byref(buf(k)), ctypes.byref(buf(v)),
+                -1 if last is not None else int(start), n, on.ptr), "KVCache8.read")
+        return k, v
+
+    def attend(self, q, *, window: int = 0, sinks: int = 0, scale=None, out=None, stream=None):
+        """q device (B,Hq,D), or (B,Hq,T,D) for the T newest positions, float32 (fp32
+        accuracy) or bfloat16, Hq a multiple of H -> o like q. Query t sees the
+        positions up to its own, len_b - T + t, with window >= 1 only those of the
+        window and the first `sinks`."""
+        torch = _torch()
+        if q.dim() not in (3, 4) or q.shape[0] != self.B or q.shape[-1] != self.D \
+                or q.shape[1] % self.H or q.shape[1] == 0:
+            raise ValueError(f"KVCache8.attend: q {tuple(q.shape)} over a cache of {self.B} "
+                             f"sequences, {self.H} heads of {self.D}")
+        Hq, T = int(q.shape[1]), int(q.shape[2]) if q.dim() == 4 else 1
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.D)
+        h, lib = self._live(), _lib.load()
+        with self._on(stream, q, out) as on:
+            if out is None:
+                out = torch.empty_like(q)
+            elif tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype:
+                raise ValueError("KVCache8.attend: out must be like q")
+            need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, int(window), int(sinks),
+                                                                on.ptr)
+            ws = on.workspace(need, self.device) if need else None
+            check(lib.gonn_hip_kvcache8_attend(
+                h, ctypes.byref(buf(q)), ctypes.byref(buf(out)), Hq, T, float(scale), int(window),
+                int(sinks), ws.data_ptr() if ws is not None else None, need, on.ptr),
+                "KVCache8.attend")
+        return out
+
+
 class DeviceMHA:
     """Device-resident multi-head attention (gonn_hip_mha_*): the forward of
     nn.MultiHeadAttention (nn/attention.go:107-148) with its four projections'
@@ -862,4 +1002,4 @@ __all__ = ["Available", "Supports", "SetAttnMode", "AttnMode", "Version", "Selft
            "FlashAttnF64BwdEx", "mask_strides", "Gemm",
            "Unary", "Binary",
            "BenchFlashAttnF64", "BenchFlashAttnF64Bwd", "attn_fwd", "attn_bwd", "attn_decode",
-           "attn_window_fwd", "attn_window_bwd", "KVCache", "DeviceMHA", "buf", "GonnHipError"]
+           "attn_window_fwd", "attn_window_bwd", "KVCache", "KVCache8", "DeviceMHA", "buf", "GonnHipError"]

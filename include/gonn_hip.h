@@ -335,6 +335,64 @@ size_t gonn_hip_kvcache_attend_causal_workspace_bytes(const gonn_kvcache* c, int
 int gonn_hip_kvcache_attend_causal(gonn_kvcache* c, const gonn_buf* q, gonn_buf* o, int T,
                                    double scale, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- KV cache in 8 bits ---------------------------------------------------
+ * New, like the cache above, at half its bytes. Positions come in blocks of 64.
+ * A block that is complete is held in e4m3 codes with one scale for its keys and
+ * one for its values, each the smallest power of two 2^e, e >= -100, that brings
+ * the largest finite magnitude of the block's 64 x D numbers to at most 448 (1
+ * where all are zero): a number is rounded to bf16 as it is appended and once
+ * more, to nearest even, as its block is completed. Infinities are then NaN. The
+ * positions of the last, incomplete block are held in bf16. What a cache holds
+ * is a function of its sequence alone, however that was appended. H is the number
+ * of key heads; queries may have a multiple of them.
+ *
+ * All calls run on `stream` and none waits for it (except where noted); the
+ * caller orders calls on different streams. Calls on one handle are not
+ * reentrant. append, truncate, read and attend can be captured in a HIP graph
+ * (lengths live on the device; a replayed append that would pass Lmax leaves that
+ * sequence as it is). After a captured append or truncate the host no longer
+ * knows the lengths: lengths, truncate and append then read them back first,
+ * which waits for `stream`.                                                */
+typedef struct gonn_kvcache8 gonn_kvcache8;
+
+/* D must be 64 or 128 (GONN_E_UNSUPPORTED otherwise). *out is NULL on failure. */
+int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D);
+int gonn_hip_kvcache8_free(gonn_kvcache8* c);
+/* The B current lengths, on the host.                                      */
+int gonn_hip_kvcache8_lengths(gonn_kvcache8* c, int* len, void* stream);
+/* k, v (B,H,T,D) GONN_F32 or GONN_BF16, both the same, 16-byte aligned; sequence
+ * b takes its first counts[b] rows (host int[B]; NULL = T). An append that would
+ * take a sequence past Lmax returns GONN_E_INVALID and writes nothing.      */
+int gonn_hip_kvcache8_append(gonn_kvcache8* c, const gonn_buf* k, const gonn_buf* v, int T,
+                             const int* counts, void* stream);
+/* Drops the positions from len[b] on (host int[B], at most the current lengths).
+ * A multiple of 64 is always allowed; another length only as far back as the bf16
+ * rows are kept, which is the start of the block before the one that the longest
+ * append so far ended in (GONN_E_UNSUPPORTED otherwise): the cache is then what
+ * it was when it had that length. In a captured call, which cannot be refused, a
+ * length further back becomes the start of its block.                       */
+int gonn_hip_kvcache8_truncate(gonn_kvcache8* c, const int* len, void* stream);
+/* k, v GONN_BF16 (B,H,count,D), 16-byte aligned: the numbers that positions
+ * start .. start + count - 1 are held as (exact in bf16), zeros where a sequence
+ * has none. start -1: the last `count` positions of each sequence, its newest in
+ * the last row.                                                            */
+int gonn_hip_kvcache8_read(gonn_kvcache8* c, gonn_buf* k, gonn_buf* v, int start, int count,
+                           void* stream);
+/* The T newest positions' queries: q, o (B,Hq,T,D), both GONN_F32 (fp32 accuracy)
+ * or both GONN_BF16, 16-byte aligned, Hq a multiple of H (query head h reads key
+ * head h / (Hq / H)). Query t stands at position i = len_b - T + t and sees
+ * positions j <= i, or with window >= 1 those of them with i - j < window or
+ * j < sinks (window 0: all, sinks ignored). A query that sees none gets o = 0.
+ * An infinity or a NaN in the cache reaches only the queries that see it.
+ * ws: gonn_hip_kvcache8_attend_workspace_bytes bytes with the same arguments,
+ * asked for beside the call (it depends on the lengths, and under a capture on
+ * Lmax).                                                                   */
+size_t gonn_hip_kvcache8_attend_workspace_bytes(const gonn_kvcache8* c, int Hq, int T, int window,
+                                                int sinks, void* stream);
+int gonn_hip_kvcache8_attend(gonn_kvcache8* c, const gonn_buf* q, gonn_buf* o, int Hq, int T,
+                             double scale, int window, int sinks, void* ws, size_t ws_bytes,
+                             void* stream);
+
 /* ---- fp64 GEMM of the backend -------------------------------------------
  * backend.Backend.Gemm (backend/backend.go:61-78) on the device: row-major
  * batched C = op(A) op(B); op(A) (m,k) stored (m,k), or (k,m) when transA;
