@@ -2021,7 +2021,7 @@ int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D)
                  ring = BH * 2 * gonn::kBlk8 * D * sizeof(uint16_t),
                  scales = round_up(BH * c.nblk * sizeof(float), 256),
                  lens = round_up((size_t)B * sizeof(int), 256);
-    const size_t bytes = 2 * codes + 2 * scales + 2 * ring + 2 * lens + 256;
+    const size_t bytes = 2 * codes + 2 * scales + 2 * ring + 3 * lens;
     if (hipMalloc(&h->mem, bytes) != hipSuccess) {
         (void)hipGetLastError();
         delete h;
@@ -2042,8 +2042,8 @@ int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D)
     uint8_t* state = p;
     c.len = (int*)take(lens);
     c.lo = (int*)take(lens);
-    c.ticket = (unsigned*)take(256);
-    hipError_t e = hipMemset(state, 0, 2 * lens + 256);
+    c.ticket = (unsigned*)take(lens);
+    hipError_t e = hipMemset(state, 0, 3 * lens);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         (void)hipFree(h->mem);

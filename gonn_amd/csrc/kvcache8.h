@@ -28,7 +28,7 @@ struct Cache8 {
     uint16_t* vt;  // (B*H, 2, D, 64) bf16: position p at (p / 64 % 2, :, p % 64)
     int* len;      // [B]
     int* lo;       // [B] first position whose bf16 row the ring still holds
-    unsigned* ticket;
+    unsigned* ticket;  // [B] workgroups of a running append that have read len
     int B, H, Lmax, D, nblk;
 };
 

@@ -298,17 +298,18 @@ def _torch():
     return torch
 
 
+_DTYPES = {}
+
+
 def _dtype_code(t):
-    torch = _torch()
-    if t.dtype == torch.float32:
-        return GONN_F32
-    if t.dtype == torch.bfloat16:
-        return GONN_BF16
-    if t.dtype == torch.int32:
-        return GONN_I32
-    if t.dtype == torch.float64:
-        return _lib.GONN_F64
-    raise TypeError(f"unsupported tensor dtype {t.dtype}")
+    if not _DTYPES:
+        torch = _torch()
+        _DTYPES.update({torch.float32: GONN_F32, torch.bfloat16: GONN_BF16,
+                        torch.int32: GONN_I32, torch.float64: _lib.GONN_F64})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported tensor dtype {t.dtype}")
+    return code
 
 
 def buf(t) -> Buf:
@@ -480,7 +481,10 @@ class _OnStream:
     """A call's device and stream, with the call's allocations on that stream;
     tensors used on a stream other than the current one are marked as used there,
     so that torch does not reuse their memory too early. The usual call, on the
-    current device and stream, switches neither."""
+    current device and stream, switches neither and looks the stream up as a plain
+    number (0.1 us; a Stream object takes 2)."""
+
+    __slots__ = ("ptr", "device", "_stream", "_enter")
 
     def __init__(self, device, stream, tensors):
         torch = _torch()
@@ -489,19 +493,19 @@ class _OnStream:
                 raise ValueError(f"tensors on {x.device} and {device}")
         if device.type != "cuda":
             raise ValueError(f"device API needs device tensors, not {device.type} ones")
-        current = torch.cuda.current_stream(device)
-        self.stream = current if stream is None else stream
-        self._enter = []
-        if device.index is not None and device.index != torch.cuda.current_device():
-            self._enter.append(torch.cuda.device(device))
-        if self.stream.cuda_stream != current.cuda_stream:
-            self._enter.append(torch.cuda.stream(self.stream))
+        self.device, self._stream, self._enter = device, stream, ()
+        here = device.index == torch.cuda.current_device()
+        current = torch._C._cuda_getCurrentRawStream(device.index)
+        self.ptr = current if stream is None else stream.cuda_stream
+        if not here:
+            self._stream = torch.cuda.current_stream(device) if stream is None else stream
+            self._enter = (torch.cuda.device(device), torch.cuda.stream(self._stream))
+        elif self.ptr != current:
+            self._enter = (torch.cuda.stream(stream),)
+        if self.ptr != current:
             for x in tensors:
                 if x is not None:
-                    x.record_stream(self.stream)
-        elif self._enter:
-            self._enter.append(torch.cuda.stream(self.stream))
-        self.ptr = ctypes.c_void_p(self.stream.cuda_stream)
+                    x.record_stream(stream)
 
     def __enter__(self):
         for c in self._enter:
@@ -512,20 +516,22 @@ class _OnStream:
         for c in reversed(self._enter):
             c.__exit__(*exc)
 
-    def workspace(self, nbytes, device):
+    def workspace(self, nbytes):
         """Workspace of one call. Inside a graph capture each call has its own,
         from the graph's pool: the shared one may grow (and move) later, and two
         graphs that share it could not run side by side."""
+        if nbytes == 0:
+            return None
         torch = _torch()
         if torch.cuda.is_current_stream_capturing():
-            return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
-        return _WS.get(nbytes, device, self.stream)
+            return torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
+        return _WS.get(nbytes, self.device, self._stream)
 
 
 def _window_shapes(what, q, k, v):
     B, H, Sq, D = _shape4(q, "q")
     Bk, Hkv, Sk, Dk = _shape4(k, "k")
-    if tuple(v.shape) != tuple(k.shape):
+    if v.shape != k.shape:
         raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     if Bk != B or Dk != D or Hkv == 0 or H % Hkv:
         raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit together")
@@ -535,7 +541,7 @@ def _window_shapes(what, q, k, v):
 
 
 def _window_like(what, name, t, ref):
-    if tuple(t.shape) != tuple(ref.shape) or t.dtype != ref.dtype:
+    if t.shape != ref.shape or t.dtype != ref.dtype:
         raise ValueError(f"{what}: {name} must be {tuple(ref.shape)} {ref.dtype}, got "
                          f"{tuple(t.shape)} {t.dtype}")
 
@@ -556,8 +562,9 @@ def attn_window_fwd(q, k, v, *, window: int, sinks: int = 0, scale=None, kv_len=
         scale = 1.0 / math.sqrt(D)
     with _OnStream(q.device, stream, (q, k, v, kv_len, out, lse_out)) as on:
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _window_like("attn_window_fwd", "out", out, q)
+            out = torch.empty_like(q)
+        else:
+            _window_like("attn_window_fwd", "out", out, q)
         if lse_out is None and lse:
             lse_out = torch.empty((B * H, Sq), dtype=torch.float32, device=q.device)
         a = WindowFwdArgs(buf(q), buf(k), buf(v), buf(out), buf(lse_out), B, H, Hkv, Sq, Sk, D,
@@ -581,15 +588,18 @@ def attn_window_bwd(q, k, v, o, lse, dO, *, window: int, sinks: int = 0, scale=N
         scale = 1.0 / math.sqrt(D)
     given = out if out is not None else ()
     with _OnStream(q.device, stream, (q, k, v, o, lse, dO, kv_len, *given)) as on:
-        dq, dk, dv = out if out is not None else (torch.empty_like(x) for x in (q, k, v))
-        for name, t, ref in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-            _window_like(what, name, t, ref)
+        if out is None:
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        else:
+            dq, dk, dv = out
+            for name, t, ref in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+                _window_like(what, name, t, ref)
         a = WindowBwdArgs(buf(q), buf(k), buf(v), buf(o), buf(lse), buf(dO), buf(dq), buf(dk),
                           buf(dv), B, H, Hkv, Sq, Sk, D, float(scale), int(window), int(sinks),
                           buf(kv_len))
         lib = _lib.load()
         nb = lib.gonn_hip_attn_workspace_bytes(GONN_OP_WINDOW_BWD, ctypes.byref(a))
-        ws = on.workspace(nb, q.device)
+        ws = on.workspace(nb)
         check(lib.gonn_hip_attn_window_bwd(ctypes.byref(a),
                                            ws.data_ptr() if ws is not None else None, nb, on.ptr),
               what)
@@ -772,9 +782,6 @@ class KVCache8:
         return self._h
 
     def _on(self, stream, *tensors):
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"KVCache8: a tensor on {t.device}, the cache on {self.device}")
         return _OnStream(self.device, stream, tensors)
 
     def _ints(self, n, what):
@@ -855,7 +862,7 @@ class KVCache8:
                 raise ValueError("KVCache8.attend: out must be like q")
             need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, int(window), int(sinks),
                                                                 on.ptr)
-            ws = on.workspace(need, self.device) if need else None
+            ws = on.workspace(need)
             check(lib.gonn_hip_kvcache8_attend(
                 h, ctypes.byref(buf(q)), ctypes.byref(buf(out)), Hq, T, float(scale), int(window),
                 int(sinks), ws.data_ptr() if ws is not None else None, need, on.ptr),
