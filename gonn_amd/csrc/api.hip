@@ -839,7 +839,7 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     const gonn::Cache8& c = h->c;
     const long long R = (long long)Hq / c.H * T, cus = gonn::device_cus();
     Plan8 p{};
-    p.rows = R <= 32 ? 32 : (R <= 64 ? 64 : 128);
+    p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
     int longest = c.Lmax;
     if (!h->captured && !stream_captures(s)) longest = *std::max_element(h->len.begin(), h->len.end());
     long long blocks = (longest + gonn::kBlk8 - 1) / gonn::kBlk8;
@@ -852,7 +852,7 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     const long long units = (long long)c.B * c.H * ((R + p.rows - 1) / p.rows);
     // Splits of 32 blocks level out sequences of different lengths; shorter ones
     // where the device has room for more workgroups, down to a block per key wave.
-    const long long want = 4 * cus, least = 128 / p.rows;
+    const long long want = 4 * cus, least = p.rows <= 32 ? 4 : 128 / p.rows;
     long long split = 32;
     if (units * ((blocks + split - 1) / split) < want)
         split = std::max(least, blocks * units / want);

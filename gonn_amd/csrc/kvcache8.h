@@ -56,7 +56,7 @@ struct Attend8 {
     float* part_ml;  // (B*Hq*T, nsplit, 2) maximum and sum, log2 units
     int Hq, T, window, sinks;  // window 0: every position
     int split, nsplit;         // blocks per split, splits at most
-    int rows;                  // rows (heads x queries) per workgroup: 32, 64 or 128
+    int rows;                  // rows (heads x queries) per workgroup: 16, 32, 64 or 128
     float scale_log2;
 };
 hipError_t launch_attend8(const Attend8& a, int is_bf16, hipStream_t s);

@@ -76,6 +76,58 @@ GONN_DEV bool sees8(int i, int j, int window, int sinks) {
     return j <= i && (window == 0 || i - j < window || j < sinks);
 }
 
+// The q operand of eight channels, and eight weights as one.
+template <int NP>
+GONN_DEV void pieces(const float* x, bf16x8* f) {
+    if constexpr (NP == 1) f[0] = pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+    else {
+        const bf16x8x3 s = split3(x);
+        f[0] = s.h;
+        f[1] = s.m;
+        f[2] = s.l;
+    }
+}
+template <int NP, typename T>
+GONN_DEV void load_q(const T* p, bf16x8* f) {
+    if constexpr (NP == 1) f[0] = *(const bf16x8*)p;
+    else {
+        const f32x4 u = *(const f32x4*)p, v = *(const f32x4*)(p + 4);
+        const float y[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        pieces<NP>(y, f);
+    }
+}
+GONN_DEV f32x4 mfma_bf16_16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Over the four lanes 16 apart.
+GONN_DEV float quad_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return pair_max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+GONN_DEV float quad_sum(float x) { return pair_sum32(pair_sum16(x)); }
+
+// Channels d .. d + 3 of a row's result: o, or one split's part of it.
+template <int D, typename T>
+GONN_DEV void write_row4(const Attend8& a, size_t row, int sp, int d, f32x4 v, float m, float l) {
+    if (a.nsplit > 1) {
+        *(f32x4*)(a.part_o + (row * a.nsplit + sp) * D + d) = v;
+        if (d == 0) {
+            // A NaN row has no maximum; a finite one keeps its weight non-zero.
+            a.part_ml[(row * a.nsplit + sp) * 2 + 0] = l != l ? 0.f : m;
+            a.part_ml[(row * a.nsplit + sp) * 2 + 1] = l;
+        }
+        return;
+    }
+    v *= l == 0.f ? 0.f : 1.f / l;
+    if constexpr (sizeof(T) == 4) *(f32x4*)((float*)a.o + row * D + d) = v;
+    else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        *(bf16x4*)((bf16*)a.o + row * D + d) =
+            bf16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+    }
+}
+
 // One element of the cache, for the plain path.
 GONN_DEV float element8(const Cache8& c, size_t bh, int len, int key, int d, bool v) {
     const int blk = key / kBlk8, r = key % kBlk8;
@@ -95,20 +147,21 @@ GONN_DEV float float_of(T x) {
     else return bf16_to_f32(__builtin_bit_cast(uint16_t, x));
 }
 
-// The wave's 32 rows in plain fp32 products, for results that are not finite: a
-// masked position's weight of 0 would make NaN of a value that is.
+// One wave's 32 rows in plain fp32 products, for results that are not finite: a
+// masked position's weight of 0 would make NaN of a value that is. 32 channels at a
+// time (few registers beside the kernels'), each time from the scores on.
 template <int D, typename T>
 GONN_DEV void attend8_plain(const Attend8& a, size_t bh, int len, const T* qrow, const Blocks8& bs,
-                            int b0, int b1, int step, int pi, f32x16* oacc, float& m, float& l) {
-    constexpr int HD = D / 2, NDT = D / 32;
+                            int b0, int b1, int pi, size_t row, int sp, bool live) {
+    constexpr int HD = D / 2;
     const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31;
-    for (int t = 0; t < NDT; t++) oacc[t] = f32x16{};
-    m = -INFINITY;
-    l = 0.f;
 #pragma unroll 1
-    for (int bi = b0; bi < b1; bi += step)
+    for (int t = 0; t < D / 32; t++) {
+        f32x16 o = f32x16{};
+        float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-        for (int kb = bs.block(bi) * kBlk8, u = 0; u < 2; u++, kb += 32) {
+        for (int x = 2 * b0; x < 2 * b1; x++) {
+            const int kb = bs.block(x >> 1) * kBlk8 + 32 * (x & 1);
             if (kb >= len) continue;
             const int kr = kb + ln < len ? kb + ln : len - 1;
             f32x16 s = f32x16{};
@@ -119,6 +172,7 @@ GONN_DEV void attend8_plain(const Attend8& a, size_t bh, int len, const T* qrow,
             for (int r = 0; r < 16; r++) {
                 const int key = kb + 8 * (r >> 2) + 4 * g + (r & 3);
                 s[r] = key < len && sees8(pi, key, a.window, a.sinks) ? s[r] * a.scale_log2 : -INFINITY;
+                // A NaN score has to make the row NaN: fmaxf would drop it.
                 mx = s[r] != s[r] ? s[r] : fmaxf(mx, s[r]);
             }
             mx = pair_max32(mx);
@@ -131,30 +185,34 @@ GONN_DEV void attend8_plain(const Attend8& a, size_t bh, int len, const T* qrow,
             }
             l = l * alpha + rs;
             m = mnew;
-            for (int t = 0; t < NDT; t++) oacc[t] *= alpha;
+            o *= alpha;
 #pragma unroll 1
-            for (int x = 0; x < 32; x++) {
-                const int r = x >> 1, h = x & 1, key = kb + 8 * (r >> 2) + 4 * h + (r & 3);
+            for (int y = 0; y < 32; y++) {
+                const int r = y >> 1, h = y & 1, key = kb + 8 * (r >> 2) + 4 * h + (r & 3);
                 float w = 0.f;
                 for (int i = 0; i < 16; i++) w = i == r ? s[i] : w;
                 const float other = __shfl_xor(w, 32);
                 w = h == g ? w : other;
                 if (key >= len) continue;  // uniform
                 const bool on = sees8(pi, key, a.window, a.sinks);
-                for (int t = 0; t < NDT; t++)
-                    for (int e = 0; e < 16; e++) {
-                        const float v = element8(a.c, bh, len, key, 32 * t + 8 * (e >> 2) + 4 * g + (e & 3), true);
-                        oacc[t][e] = on ? __builtin_fmaf(w, v, oacc[t][e]) : oacc[t][e];
-                    }
+                for (int e = 0; e < 16; e++) {
+                    const float v = element8(a.c, bh, len, key, 32 * t + 8 * (e >> 2) + 4 * g + (e & 3), true);
+                    o[e] = on ? __builtin_fmaf(w, v, o[e]) : o[e];
+                }
             }
         }
-    l = pair_sum32(l);
+        l = pair_sum32(l);
+        if (live)
+            for (int rq = 0; rq < 4; rq++)
+                write_row4<D, T>(a, row, sp, t * 32 + rq * 8 + g * 4,
+                                 f32x4{o[rq * 4], o[rq * 4 + 1], o[rq * 4 + 2], o[rq * 4 + 3]}, m, l);
+    }
 }
 
 }  // namespace
 
 template <int D, typename T, int WQ>
-__global__ __launch_bounds__(256, 1) void attend8_kernel(Attend8 a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attend8_kernel(Attend8 a) {
     constexpr int WK = 4 / WQ, BM = WQ * 32, NP = sizeof(T) == 4 ? 3 : 1;
     constexpr int NJ = D / 32, NDT = D / 32;  // 32-element steps of a row, channel tiles
     constexpr int NE = 16 * NDT + 2;
@@ -194,18 +252,7 @@ __global__ __launch_bounds__(256, 1) void attend8_kernel(Attend8 a) {
     // q operand of step (j, x): elements 32 j + 16 g + 8 x .. +7.
     bf16x8 qf[NJ * 2][NP];
     for (int j = 0; j < NJ; j++)
-        for (int x = 0; x < 2; x++) {
-            const T* p = qrow + 32 * j + 16 * g + 8 * x;
-            if constexpr (NP == 1) qf[2 * j + x][0] = *(const bf16x8*)p;
-            else {
-                const f32x4 u = *(const f32x4*)p, v = *(const f32x4*)(p + 4);
-                const float y[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-                const bf16x8x3 s = split3(y);
-                qf[2 * j + x][0] = s.h;
-                qf[2 * j + x][1] = s.m;
-                qf[2 * j + x][2] = s.l;
-            }
-        }
+        for (int x = 0; x < 2; x++) load_q<NP>(qrow + 32 * j + 16 * g + 8 * x, qf[2 * j + x]);
     // Cache row of operand row ln: accumulator register r of half g is then
     // position 16 g + r of the 32-position tile.
     const int krow = 16 * ((ln >> 2) & 1) + 4 * (ln >> 3) + (ln & 3);
@@ -273,14 +320,7 @@ __global__ __launch_bounds__(256, 1) void attend8_kernel(Attend8 a) {
                     e[j] = fast_exp2(s[u][8 * x + j] - mref);
                     rs[j & 3] += e[j];
                 }
-                if constexpr (NP == 1) {
-                    pf[u][x][0] = pack8(e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]);
-                } else {
-                    const bf16x8x3 p = split3(e);
-                    pf[u][x][0] = p.h;
-                    pf[u][x][1] = p.m;
-                    pf[u][x][2] = p.l;
-                }
+                pieces<NP>(e, pf[u][x]);
             }
         l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     };
@@ -349,7 +389,6 @@ __global__ __launch_bounds__(256, 1) void attend8_kernel(Attend8 a) {
 
     auto merge = [&](float& l) {
         if constexpr (WK > 1) {
-            __syncthreads();
             if (wk > 0) {
                 float* d = red + ((wk - 1) * WQ + wq) * NE * 64 + lane;
                 for (int t = 0; t < NDT; t++)
@@ -380,32 +419,213 @@ __global__ __launch_bounds__(256, 1) void attend8_kernel(Attend8 a) {
         if (__builtin_amdgcn_ballot_w64(bad && ri < R) && lane == 0) again = 1;
     }
     __syncthreads();
-    if (again) {  // uniform
-        attend8_plain<D>(a, bh, len, qrow, bs, b0 + wk, b1, WK, pi, oacc, m, lt);
-        merge(lt);
-    }
-    if (wk > 0 || ri >= R) return;
+    if (wk > 0) return;
     const size_t row = (size_t)bh * R + ri;
-    const bool whole = a.nsplit == 1;
-    const float inv = whole ? (lt == 0.f ? 0.f : 1.f / lt) : 1.f;
+    if (again) {  // uniform
+        attend8_plain<D>(a, bh, len, qrow, bs, b0, b1, pi, row, sp, ri < R);
+        return;
+    }
+    if (ri >= R) return;
     for (int t = 0; t < NDT; t++)
-        for (int rq = 0; rq < 4; rq++) {
-            f32x4 v;
-            for (int i = 0; i < 4; i++) v[i] = oacc[t][rq * 4 + i] * inv;
-            const int d = t * 32 + rq * 8 + g * 4;
-            if (!whole) *(f32x4*)(a.part_o + (row * a.nsplit + sp) * D + d) = v;
-            else if constexpr (NP == 3) *(f32x4*)((float*)a.o + row * D + d) = v;
-            else {
-                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-                *(bf16x4*)((bf16*)a.o + row * D + d) =
-                    bf16x4{to_bf16(v[0]), to_bf16(v[1]), to_bf16(v[2]), to_bf16(v[3])};
+        for (int rq = 0; rq < 4; rq++)
+            write_row4<D, T>(a, row, sp, t * 32 + rq * 8 + g * 4,
+                             f32x4{oacc[t][rq * 4], oacc[t][rq * 4 + 1], oacc[t][rq * 4 + 2], oacc[t][rq * 4 + 3]},
+                             m, lt);
+}
+
+// Up to 16 rows (a decoding step, with up to 16 query heads to a key head): the
+// same scheme on v_mfma_f32_16x16x32_bf16, four key waves. It costs half the
+// products, weights and accumulators of a 32-row tile, and reads whole runs: an
+// operand of V^T is 16 channels x 64 bytes, 1 KB in a row.
+//
+// Bound: the cache stream. Lane l of a wave holds row n = l % 16 and quarter g = l /
+// 16 of the keys: position 16 g + 4 u + r of the block in register r of tile u.
+template <int D, typename T>
+__global__ __launch_bounds__(256, 2) void attend8_few_kernel(Attend8 a) {
+    constexpr int WK = 4, NP = sizeof(T) == 4 ? 3 : 1, NJ = D / 64, ND = D / 16;
+    constexpr int NE = 4 * ND + 2;
+    __shared__ float red[(WK - 1) * NE * 64];
+    __shared__ int again;
+
+    const Cache8& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wk = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
+    const int T_ = a.T, R = a.Hq / c.H * T_, BH = c.B * c.H;
+    int us, rb;
+    map_block(blockIdx.x, 1, BH * a.nsplit, false, us, rb, 1, true);
+    const int sp = __builtin_amdgcn_readfirstlane(us / BH), bhi = us - sp * BH, b = bhi / c.H;
+    const size_t bh = bhi;
+    int len = c.len[b];
+    len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
+    int t0, t1;
+    query_span(0, R - 1, T_, t0, t1);
+    Blocks8 bs;
+    bs.init(len - T_ + t0, len - T_ + t1, a.window, a.sinks);
+    const int nv = bs.count(), ns = splits8(a, nv);
+    if (sp >= ns && sp > 0) return;  // uniform; split 0 writes also where there is nothing to see
+    const int b0 = ns ? (int)((long long)sp * nv / ns) : 0;
+    const int b1 = ns ? (int)((long long)(sp + 1) * nv / ns) : 0;
+    const int closed = len / kBlk8;
+    const int open_at = b1 > b0 && bs.block(b1 - 1) == closed ? b1 - 1 : b1;
+
+    // Block's operands: tile u's K rows, 64 jj + 16 g .. of their channels; V^T rows
+    // 16 t + n, positions 16 g ...
+    const int krow = 16 * (n >> 2) + (n & 3);
+    u32x4 kr[4][NJ], vr[ND];
+    float ksc = 0.f, vsc = 0.f;
+    auto load_k = [&](int blk) {
+        const uint8_t* p = c.k8 + ((bh * c.nblk + blk) * kBlk8 + krow) * D + 16 * g;
+        for (int u = 0; u < 4; u++)
+            for (int j = 0; j < NJ; j++)
+                kr[u][j] = __builtin_nontemporal_load((const u32x4*)(p + 4 * u * D + 64 * j));
+        ksc = c.ks[bh * c.nblk + blk];
+    };
+    auto load_v = [&](int blk) {
+        const uint8_t* p = c.v8 + ((bh * c.nblk + blk) * D + n) * kBlk8 + 16 * g;
+        for (int t = 0; t < ND; t++)
+            vr[t] = __builtin_nontemporal_load((const u32x4*)(p + t * 16 * kBlk8));
+        vsc = c.vs[bh * c.nblk + blk];
+    };
+    int bi = b0 + wk;
+    if (bi < open_at) {
+        load_k(bs.block(bi));
+        load_v(bs.block(bi));
+    }
+    const int rc = n < R ? n : R - 1, pi = len - T_ + rc % T_;
+    const int pw0 = len - T_ + t0, pw1 = len - T_ + t1;
+    const T* qrow = (const T*)a.q + ((size_t)bh * R + rc) * D;
+    bf16x8 qf[2 * NJ][NP];
+    for (int j = 0; j < NJ; j++)
+        for (int x = 0; x < 2; x++) load_q<NP>(qrow + 64 * j + 16 * g + 8 * x, qf[2 * j + x]);
+    if (tid == 0) again = 0;
+
+    f32x4 oacc[ND];
+    for (int t = 0; t < ND; t++) oacc[t] = f32x4{};
+    float m = -INFINITY, l = 0.f;
+
+    // A whole block: kf(u, jj, x) and vf(t, w) give the operands.
+    auto block = [&](int blk, auto kf, auto vf, auto next_k, auto next_v) {
+        f32x4 s[4];
+        for (int u = 0; u < 4; u++) {
+            f32x4 x0 = f32x4{}, x1 = f32x4{};
+            for (int j = 0; j < NJ; j++)
+                for (int x = 0; x < 2; x++) {
+                    const bf16x8 k = kf(u, j, x);
+                    if constexpr (NP == 3) {
+                        x1 = mfma_bf16_16(k, qf[2 * j + x][2], x1);
+                        x1 = mfma_bf16_16(k, qf[2 * j + x][1], x1);
+                    }
+                    x0 = mfma_bf16_16(k, qf[2 * j + x][0], x0);
+                }
+            if constexpr (NP == 3) x0 += x1;
+            s[u] = x0 * a.scale_log2;
+        }
+        for (int u = 0; u < 4; u++) pin_before_branch(s[u]);
+        next_k();
+        const int k0 = blk * kBlk8;
+        if (!(k0 + 63 <= pw0 && (a.window == 0 || pw1 - k0 < a.window || k0 + 63 < a.sinks)))
+            for (int u = 0; u < 4; u++)
+                for (int r = 0; r < 4; r++)
+                    s[u][r] = sees8(pi, k0 + 16 * g + 4 * u + r, a.window, a.sinks) ? s[u][r] : -INFINITY;
+        float mx = -INFINITY;
+        for (int u = 0; u < 4; u++)
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, s[u][r]);
+        mx = quad_max(mx);
+        const bool need = mx > m && (m == -INFINITY || mx - m > 8.f);
+        if (__builtin_amdgcn_ballot_w64(need)) {
+            const float mn = need ? mx : m;
+            const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+            m = mn;
+            l *= alpha;
+            for (int t = 0; t < ND; t++) oacc[t] *= alpha;
+        }
+        const float mref = m == -INFINITY ? 0.f : m;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+        bf16x8 pf[2][NP];  // positions 16 g + 8 w ..
+        for (int w = 0; w < 2; w++) {
+            float e[8];
+            for (int i = 0; i < 8; i++) {
+                e[i] = fast_exp2(s[2 * w + (i >> 2)][i & 3] - mref);
+                rs[i & 3] += e[i];
+            }
+            pieces<NP>(e, pf[w]);
+        }
+        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        for (int t = 0; t < ND; t++) {
+            if constexpr (NP == 1) {
+                for (int w = 0; w < 2; w++) oacc[t] = mfma_bf16_16(vf(t, w), pf[w][0], oacc[t]);
+            } else {
+                f32x4 y = f32x4{};
+                const bf16x8 v[2] = {vf(t, 0), vf(t, 1)};
+                for (int i = NP - 1; i >= 0; i--)
+                    for (int w = 0; w < 2; w++) y = mfma_bf16_16(v[w], pf[w][i], y);
+                oacc[t] += y;
             }
         }
-    if (!whole && g == 0) {
-        // A NaN row has no maximum; a finite one keeps its weight non-zero.
-        a.part_ml[(row * a.nsplit + sp) * 2 + 0] = lt != lt ? 0.f : m;
-        a.part_ml[(row * a.nsplit + sp) * 2 + 1] = lt;
+        for (int t = 0; t < ND; t++) pin_before_branch(oacc[t]);
+        next_v();
+    };
+    for (; bi < open_at; bi += WK) {
+        const int blk = bs.block(bi), nx = bi + WK < open_at ? bs.block(bi + WK) : blk;
+        const float k1 = ksc, v1 = vsc;
+        block(
+            blk, [&](int u, int j, int x) { return decode8(kr[u][j][2 * x], kr[u][j][2 * x + 1], k1); },
+            [&](int t, int w) { return decode8(vr[t][2 * w], vr[t][2 * w + 1], v1); },
+            [&] { load_k(nx); }, [&] { load_v(nx); });
     }
+    if (open_at < b1 && (open_at - b0) % WK == wk) {
+        // The open block, bf16; positions past the last are no one's values.
+        const uint16_t* kp = c.kt + ((bh * 2 + (closed & 1)) * kBlk8 + krow) * D + 16 * g;
+        const uint16_t* vp = c.vt + ((bh * 2 + (closed & 1)) * D + n) * kBlk8 + 16 * g;
+        const int left = len - closed * kBlk8 - 16 * g;
+        block(
+            closed,
+            [&](int u, int j, int x) { return *(const bf16x8*)(kp + 4 * u * D + 64 * j + 8 * x); },
+            [&](int t, int w) {
+                u16x8 v = *(const u16x8*)(vp + (size_t)t * 16 * kBlk8 + 8 * w);
+                for (int e = 0; e < 8; e++) v[e] = 8 * w + e < left ? v[e] : (uint16_t)0;
+                return __builtin_bit_cast(bf16x8, v);
+            },
+            [] {}, [] {});
+    }
+
+    float lt = quad_sum(l);
+    __syncthreads();
+    if (wk > 0) {
+        float* d = red + (wk - 1) * NE * 64 + lane;
+        for (int t = 0; t < ND; t++)
+            for (int r = 0; r < 4; r++) d[(t * 4 + r) * 64] = oacc[t][r];
+        d[(NE - 2) * 64] = m;
+        d[(NE - 1) * 64] = lt;
+    }
+    __syncthreads();
+    if (wk == 0) {
+        for (int w = 1; w < WK; w++) {
+            const float* d = red + (w - 1) * NE * 64 + lane;
+            const float m2 = d[(NE - 2) * 64], l2 = d[(NE - 1) * 64];
+            const float M = fmaxf(m, m2), Mr = M == -INFINITY ? 0.f : M;
+            const float x = fast_exp2(m - Mr), y = fast_exp2(m2 - Mr);
+            lt = lt * x + l2 * y;
+            for (int t = 0; t < ND; t++)
+                for (int r = 0; r < 4; r++) oacc[t][r] = oacc[t][r] * x + d[(t * 4 + r) * 64] * y;
+            m = M;
+        }
+        bool bad = nonfinite(lt);
+        for (int t = 0; t < ND; t++)
+            for (int r = 0; r < 4; r++) bad |= nonfinite(oacc[t][r]);
+        if (__builtin_amdgcn_ballot_w64(bad && n < R) && lane == 0) again = 1;
+    }
+    __syncthreads();
+    if (wk > 0) return;
+    const size_t row = (size_t)bh * R;
+    if (again) {  // uniform: one wave, the 32-row form
+        const int ln = lane & 31, ri = ln < R ? ln : R - 1;
+        attend8_plain<D>(a, bh, len, (const T*)a.q + (row + ri) * D, bs, b0, b1, len - T_ + ri % T_,
+                         row + ln, sp, ln < R);
+        return;
+    }
+    if (n >= R) return;
+    for (int t = 0; t < ND; t++) write_row4<D, T>(a, row + n, sp, t * 16 + 4 * g, oacc[t], m, lt);
 }
 
 // Splits of one row joined: one workgroup of D threads per row. A split in which
@@ -447,7 +667,8 @@ void run_attend8(const Attend8& a, hipStream_t s) {
     const int R = a.Hq / a.c.H * a.T;
     const unsigned rows = (unsigned)(a.c.B * a.c.H) * (unsigned)R;
     const unsigned grid = (unsigned)((R + a.rows - 1) / a.rows) * (unsigned)(a.c.B * a.c.H) * (unsigned)a.nsplit;
-    if (a.rows == 32) attend8_kernel<D, T, 1><<<grid, 256, 0, s>>>(a);
+    if (a.rows == 16) attend8_few_kernel<D, T><<<grid, 256, 0, s>>>(a);
+    else if (a.rows == 32) attend8_kernel<D, T, 1><<<grid, 256, 0, s>>>(a);
     else if (a.rows == 64) attend8_kernel<D, T, 2><<<grid, 256, 0, s>>>(a);
     else attend8_kernel<D, T, 4><<<grid, 256, 0, s>>>(a);
     if (a.nsplit > 1) attend8_combine_kernel<D, T><<<rows, D, 0, s>>>(a);

@@ -1,7 +1,8 @@
 """Wait states between MFMAs and the first use of their results, over every path (CPU).
 
 A VALU or memory instruction may read or overwrite an MFMA's result only some wait states
-after it: 11 for v_mfma_f32_32x32x16_bf16, 18 for v_mfma_f32_32x32x2_f32 (an MFMA that
+after it: 7 for v_mfma_f32_16x16x32_bf16, 11 for
+32x32x16, 18 for v_mfma_f32_32x32x2_f32 (an MFMA that
 accumulates onto it needs none). The compiler inserts them, but where it sank the reading
 instructions below a branch it has inserted too few on the taken path, and the last
 registers of a result were read before they were written. pin_before_branch (common.h)
@@ -27,7 +28,7 @@ def _regs(text):
 
 
 def _need(op):
-    return 18 if "32x32x2_f32" in op else 11
+    return 18 if "32x32x2_f32" in op else 7 if "16x16x32" in op else 11
 
 
 def _parse(t):
