@@ -405,6 +405,9 @@ int check_window(const A* a, gonn::WindowParams* p) {
     p->sinks = std::min(a->sinks, a->Sk);
     p->scale = (float)a->scale;
     p->scale_log2 = (float)(a->scale * 1.4426950408889634);
+    const QFold qf = q_fold(a->scale);
+    p->c2 = qf.c2;
+    p->sign = qf.sign;
     p->kv_len = a->kv_len.ptr ? (const int*)a->kv_len.ptr : nullptr;
     return GONN_OK;
 }
@@ -427,14 +430,17 @@ int check_window_bwd(const gonn_attn_window_bwd_args* a, gonn::WindowParams* p) 
     return GONN_OK;
 }
 
-// delta, then the dK/dV partials; fills p's work items and, given ws, its pointers.
+// lse2 and delta, then the dK/dV partials; fills p's work items and, given ws, its
+// pointers.
 size_t window_bwd_ws(gonn::WindowParams& p, int D, int is_bf16, void* ws) {
-    const size_t delta = round_up((size_t)p.B * p.H * p.Sq * sizeof(float), 256);
+    p.Sp = (int)round_up((size_t)p.Sq, 64);
+    const size_t rows = round_up((size_t)p.B * p.H * p.Sp * sizeof(float), 256);
     const size_t part = gonn::plan_window_bwd(p, D, is_bf16);
     uint8_t* w = (uint8_t*)round_up((size_t)ws, 256);
-    p.delta = (float*)w;
-    p.part = (float*)(w + delta);
-    return delta + part + 256;
+    p.lse2 = (float*)w;
+    p.delta = (float*)(w + rows);
+    p.part = (float*)(w + 2 * rows);
+    return 2 * rows + part + 256;
 }
 
 // ---- helpers for the host shims ----------------------------------------

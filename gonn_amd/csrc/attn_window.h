@@ -176,17 +176,15 @@ GONN_DEV Frag<NP> tile_col(const SplitTile<D>& tl, char* tile, int w, int ks, in
     return f;
 }
 
-// acc[t][r] += w * row[32 t + 8 (r / 4) + 4 g + r % 4] where on, untouched where
-// not: a product that an infinity or a NaN in a masked place cannot reach.
-template <int D, typename T>
-GONN_DEV void add_row(f32x16* acc, float w, const T* row, int g, bool on) {
+// acc[r] += w * row[8 (r / 4) + 4 g + r % 4] where on, untouched where not: a product
+// that an infinity or a NaN in a masked place cannot reach.
+template <typename T>
+GONN_DEV void add_row32(f32x16& acc, float w, const T* row, int g, bool on) {
 #pragma unroll
-    for (int t = 0; t < D / 32; t++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const float x = to_float(row[32 * t + 8 * (r >> 2) + 4 * g + (r & 3)]);
-            acc[t][r] = on ? __builtin_fmaf(w, x, acc[t][r]) : acc[t][r];
-        }
+    for (int r = 0; r < 16; r++) {
+        const float x = to_float(row[8 * (r >> 2) + 4 * g + (r & 3)]);
+        acc[r] = on ? __builtin_fmaf(w, x, acc[r]) : acc[r];
+    }
 }
 // Weight r of the 32 that a wave holds per column (16 in each half): key or
 // query row 8 (r / 4) + 4 h + r % 4.

@@ -12,64 +12,77 @@ namespace gonn {
 
 namespace {
 
-// The wave's 32 rows over this key wave's stages in plain fp32 products from
-// global memory, for rows whose result is not finite (or, in fp32, outside the
-// split's range): a masked key's weight of 0 would make NaN of an infinite V, so
-// tiles that some row does not see in full add P V with a select per key.
+// O of four channels and LSE of a row.
 template <int D, typename T>
-GONN_DEV void window_fwd_plain(const WindowParams& p, const T* qrow, const T* Kg, const T* Vg,
-                               const KeyStages& ks, int BN, int off, int kl, const Band& band,
-                               int qw, int qi, f32x16* oacc, float& m, float& l) {
-    constexpr int HD = D / 2, NDT = D / 32;
-    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31;
-    for (int t = 0; t < NDT; t++) oacc[t] = f32x16{};
-    m = -INFINITY;
-    l = 0.f;
-#pragma unroll 1
-    for (int st = 0; st < ks.count(); st++) {
-        const int kb = ks.stage(st) * BN + off;
-        if (kb >= kl || !band.any(qw, qw + 31, kb, kb + 31)) continue;  // wave-uniform
-        const T* krow = Kg + (size_t)(kb + ln < kl ? kb + ln : kl - 1) * D + g * HD;
-        f32x16 s = f32x16{};
-#pragma unroll 4
-        for (int i = 0; i < HD; i++)
-            s = mfma_f32(to_float(krow[i]), to_float(qrow[g * HD + i]), s);
-        float mx = -INFINITY;
-        for (int r = 0; r < 16; r++) {
-            const int key = kb + 8 * (r >> 2) + 4 * g + (r & 3);
-            s[r] = key < kl && band.sees(qi, key) ? s[r] * p.scale_log2 : -INFINITY;
-            // A NaN score has to make the row NaN: fmaxf would drop it.
-            mx = s[r] != s[r] ? s[r] : fmaxf(mx, s[r]);
-        }
-        mx = pair_max32(mx);
-        const float mnew = fmaxf(m, mx), mref = mnew == -INFINITY ? 0.f : mnew;
-        const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mref);
-        float rs = 0.f;
-        for (int r = 0; r < 16; r++) {
-            s[r] = fast_exp2(s[r] - mref);
-            rs += s[r];
-        }
-        l = l * alpha + rs;
-        m = mnew;
-        for (int t = 0; t < NDT; t++) oacc[t] *= alpha;
-        if (kb + 32 <= kl && band.all(qw, qw + 31, kb, kb + 31)) {
-#pragma unroll 1
-            for (int r = 0; r < 16; r++) {
-                const T* v = Vg + (size_t)(kb + 8 * (r >> 2) + 4 * g + (r & 3)) * D + ln;
-                const float w = weight_of(s, r, g, g);
-                for (int t = 0; t < NDT; t++) oacc[t] = mfma_f32(to_float(v[t * 32]), w, oacc[t]);
-            }
-            continue;
-        }
-#pragma unroll 1
-        for (int x = 0; x < 32; x++) {
-            const int r = x >> 1, h = x & 1, key = kb + 8 * (r >> 2) + 4 * h + (r & 3);
-            const float w = weight_of(s, r, h, g);
-            if (key >= kl) continue;  // uniform
-            add_row<D>(oacc, w, Vg + (size_t)key * D, g, band.sees(qi, key));
-        }
+GONN_DEV void write_row(const WindowParams& p, size_t row, int d, f32x4 v, float m, float l) {
+    v *= l == 0.f ? 0.f : 1.f / l;
+    store4<T>((T*)p.o + row * D + d, v);
+    // In double: m and log2 l may be large and cancel.
+    if (p.lse && d == 0) {
+        const int ex = __builtin_amdgcn_frexp_expf(l);
+        const float lm = fast_log2(__builtin_amdgcn_frexp_mantf(l));
+        p.lse[row] = l == 0.f ? -INFINITY : (float)(((double)m + (double)ex + lm) * kLn2d);
     }
-    l = pair_sum32(l);
+}
+
+// A wave's 32 rows in plain fp32 products from global memory, for rows whose result
+// is not finite (or, in fp32, outside the split's range): a masked key's weight of 0
+// would make NaN of an infinite V, so P V is added with a select per key. 32 channels
+// at a time, each time from the scores on: few registers beside the kernels'.
+template <int D, typename T>
+GONN_DEV void window_fwd_plain(const WindowParams& p, int bh, int bk, int kl, const Band& band,
+                               int qw) {
+    constexpr int HD = D / 2;
+    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31, qi = qw + ln;
+    const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
+    const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
+    const size_t row = (size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1);
+    const T* qrow = (const T*)p.q + row * D + g * HD;
+    KeyStages ks;
+    ks.init(qw, qw + 32 < p.Sq ? qw + 32 : p.Sq, kl, 32, band);
+#pragma unroll 1
+    for (int t = 0; t < D / 32; t++) {
+        f32x16 o = f32x16{};
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+        for (int st = 0; st < ks.count(); st++) {
+            const int kb = ks.stage(st) * 32;
+            const T* krow = Kg + (size_t)(kb + ln < kl ? kb + ln : kl - 1) * D + g * HD;
+            f32x16 s = f32x16{};
+#pragma unroll 4
+            for (int i = 0; i < HD; i++) s = mfma_f32(to_float(krow[i]), to_float(qrow[i]), s);
+            float mx = -INFINITY;
+            for (int r = 0; r < 16; r++) {
+                const int key = kb + 8 * (r >> 2) + 4 * g + (r & 3);
+                s[r] = key < kl && band.sees(qi, key) ? s[r] * p.scale_log2 : -INFINITY;
+                // A NaN score has to make the row NaN: fmaxf would drop it.
+                mx = s[r] != s[r] ? s[r] : fmaxf(mx, s[r]);
+            }
+            mx = pair_max32(mx);
+            const float mnew = fmaxf(m, mx), mref = mnew == -INFINITY ? 0.f : mnew;
+            const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - mref);
+            float rs = 0.f;
+            for (int r = 0; r < 16; r++) {
+                s[r] = fast_exp2(s[r] - mref);
+                rs += s[r];
+            }
+            l = l * alpha + rs;
+            m = mnew;
+            o *= alpha;
+#pragma unroll 1
+            for (int x = 0; x < 32; x++) {
+                const int r = x >> 1, h = x & 1, key = kb + 8 * (r >> 2) + 4 * h + (r & 3);
+                const float w = weight_of(s, r, h, g);
+                if (key >= kl) continue;  // uniform
+                add_row32(o, w, Vg + (size_t)key * D + 32 * t, g, band.sees(qi, key));
+            }
+        }
+        l = pair_sum32(l);
+        if (qi < p.Sq)
+            for (int rq = 0; rq < 4; rq++)
+                write_row<D, T>(p, row, 32 * t + 8 * rq + 4 * g,
+                                f32x4{o[4 * rq], o[4 * rq + 1], o[4 * rq + 2], o[4 * rq + 3]}, m, l);
+    }
 }
 
 }  // namespace
@@ -83,7 +96,6 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
     constexpr int NE = 16 * NDT + 2;
     constexpr uint32_t RED = (WK - 1) * WQ * NE * 256;
     __shared__ __attribute__((aligned(16))) char smem[NBUF * STAGE > RED ? NBUF * STAGE : RED];
-    __shared__ int again;  // some row needs the plain products
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -103,7 +115,6 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
     Stage in;
     in.init(tid);
     if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
-    if (tid == 0) again = 0;
     const T* qrow = (const T*)p.q + ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1)) * D;
     Frag<NP> qf[NKS];
     load_row_frags<D>(qrow, g, true, qf);
@@ -196,38 +207,26 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
     };
     float lt = pair_sum32(l);
     merge(lt);
-    if (wk == 0) {
-        bool bad = nonfinite(lt);
-        SplitCheck chk;
-        for (int t = 0; t < NDT; t++)
-            for (int r = 0; r < 16; r++) {
-                if constexpr (NP == 3) chk.add(oacc[t][r]);
-                else bad |= nonfinite(oacc[t][r]);
-            }
-        if constexpr (NP == 3) bad |= chk.plain();
-        if (__builtin_amdgcn_ballot_w64(bad && qi < p.Sq) && lane == 0) again = 1;
-    }
-    __syncthreads();
-    if (again) {  // uniform
-        window_fwd_plain<D>(p, qrow, Kg, Vg, ks, BN, wk * 32, kl, band, qw, qi, oacc, m, lt);
-        merge(lt);
-    }
-    if (wk > 0 || qi >= p.Sq) return;
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    T* orow = (T*)p.o + ((size_t)bh * p.Sq + qi) * D;
+    if (wk > 0) return;
+    bool bad = nonfinite(lt);
+    SplitCheck chk;
     for (int t = 0; t < NDT; t++)
-        for (int rq = 0; rq < 4; rq++) {
-            f32x4 v;
-            for (int i = 0; i < 4; i++) v[i] = oacc[t][rq * 4 + i] * inv;
-            store4<T>(orow + t * 32 + rq * 8 + g * 4, v);
+        for (int r = 0; r < 16; r++) {
+            if constexpr (NP == 3) chk.add(oacc[t][r]);
+            else bad |= nonfinite(oacc[t][r]);
         }
-    // In double: m and log2 l may be large and cancel.
-    if (p.lse && g == 0) {
-        const int ex = __builtin_amdgcn_frexp_expf(lt);
-        const float lm = fast_log2(__builtin_amdgcn_frexp_mantf(lt));
-        p.lse[(size_t)bh * p.Sq + qi] =
-            lt == 0.f ? -INFINITY : (float)(((double)m + (double)ex + lm) * kLn2d);
+    if constexpr (NP == 3) bad |= chk.plain();
+    if (__builtin_amdgcn_ballot_w64(bad && qi < p.Sq)) {
+        window_fwd_plain<D, T>(p, bh, bk, kl, band, qw);
+        return;
     }
+    if (qi >= p.Sq) return;
+    const size_t row = (size_t)bh * p.Sq + qi;
+    for (int t = 0; t < NDT; t++)
+        for (int rq = 0; rq < 4; rq++)
+            write_row<D, T>(p, row, t * 32 + rq * 8 + g * 4,
+                            f32x4{oacc[t][rq * 4], oacc[t][rq * 4 + 1], oacc[t][rq * 4 + 2],
+                                  oacc[t][rq * 4 + 3]}, m, lt);
 }
 
 namespace {

@@ -38,24 +38,26 @@ GONN_DEV void plain_products(const T* a1, const T* b1, const T* a2, const T* b2,
     }
 }
 
-// dQ of the wave's 32 queries once more in plain fp32 products (see
-// window_fwd_plain), every key stage of the block.
+// dQ of a wave's 32 queries in plain fp32 products, for results that are not finite
+// (see window_fwd_plain), 32 channels at a time.
 template <int D, typename T>
-GONN_DEV void window_dq_plain(const WindowParams& p, const T* qrow, const T* grow, const T* Kg,
-                              const T* Vg, const KeyStages& ks, int BN, int kl, const Band& band,
-                              int qw, int qi, float lq, float dl, f32x16* acc) {
-    constexpr int NDT = D / 32;
-    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31;
-    for (int t = 0; t < NDT; t++) acc[t] = f32x16{};
+GONN_DEV void window_dq_plain(const WindowParams& p, int bh, int bk, int kl, const Band& band,
+                              int qw, float lq, float dl) {
+    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31, qi = qw + ln;
+    const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
+    const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
+    const size_t row = ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1)) * D;
+    KeyStages ks;
+    ks.init(qw, qw + 32 < p.Sq ? qw + 32 : p.Sq, kl, 32, band);
 #pragma unroll 1
-    for (int st = 0; st < ks.count(); st++)
+    for (int t = 0; t < D / 32; t++) {
+        f32x16 acc = f32x16{};
 #pragma unroll 1
-        for (int off = 0; off < BN; off += 32) {
-            const int kb = ks.stage(st) * BN + off;
-            if (kb >= kl || !band.any(qw, qw + 31, kb, kb + 31)) continue;
+        for (int st = 0; st < ks.count(); st++) {
+            const int kb = ks.stage(st) * 32;
             const size_t kr = (size_t)(kb + ln < kl ? kb + ln : kl - 1) * D;
             f32x16 s, dp;
-            plain_products<D>(Kg + kr, qrow, Vg + kr, grow, g, s, dp);
+            plain_products<D>(Kg + kr, (const T*)p.q + row, Vg + kr, (const T*)p.dO + row, g, s, dp);
             for (int r = 0; r < 16; r++) {
                 const int key = kb + 8 * (r >> 2) + 4 * g + (r & 3);
                 const float pv = fast_exp2(__builtin_fmaf(s[r], p.scale_log2, -lq));
@@ -66,9 +68,16 @@ GONN_DEV void window_dq_plain(const WindowParams& p, const T* qrow, const T* gro
                 const int r = x >> 1, h = x & 1, key = kb + 8 * (r >> 2) + 4 * h + (r & 3);
                 const float w = weight_of(s, r, h, g);
                 if (key >= kl) continue;  // uniform
-                add_row<D>(acc, w, Kg + (size_t)key * D, g, band.sees(qi, key));
+                add_row32(acc, w, Kg + (size_t)key * D + 32 * t, g, band.sees(qi, key));
             }
         }
+        if (qi < p.Sq)
+            for (int rq = 0; rq < 4; rq++) {
+                f32x4 v;
+                for (int i = 0; i < 4; i++) v[i] = acc[rq * 4 + i] * p.scale;
+                store4<T>((T*)p.dq + row + 32 * t + 8 * rq + 4 * g, v);
+            }
+    }
 }
 
 }  // namespace
@@ -114,7 +123,11 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
     }
     dl = pair_sum32(dl);
     const float lq = lse_log2(p.lse_in[qr]);
-    if (ws == 0 && g == 0 && qi < p.Sq) p.delta[qr] = dl;
+    if (ws == 0 && g == 0 && qi < p.Sp) {
+        const size_t x = (size_t)bh * p.Sp + qi;
+        p.lse2[x] = qi < p.Sq ? lq : INFINITY;
+        p.delta[x] = qi < p.Sq ? dl : 0.f;
+    }
     SplitTile<D> tl;
     tl.init(lane);
 
@@ -168,8 +181,10 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
                 else bad |= nonfinite(acc[t][r]);
             }
         if constexpr (NP == 3) bad = chk.plain();
-        if (__builtin_amdgcn_ballot_w64(bad && qi < p.Sq))
-            window_dq_plain<D>(p, qrow, grow, Kg, Vg, ks, BN, kl, band, qw, qi, lq, dl, acc);
+        if (__builtin_amdgcn_ballot_w64(bad && qi < p.Sq)) {
+            window_dq_plain<D, T>(p, bh, bk, kl, band, qw, lq, dl);
+            return;
+        }
     }
     if (qi >= p.Sq) return;
     T* out = (T*)p.dq + qr * D;
@@ -195,42 +210,89 @@ struct BlockSteps {
     }
 };
 
-// dV and dK of the wave's 32 keys over steps [s0, s1), plain fp32 products.
+// One workgroup's share of the dK/dV grid: chunk c of key block kb of slice bk.
+struct DkdvItem {
+    int bk, slot, kb, c, per, b, hk, G, kl;
+    GONN_DEV void init(const WindowParams& p) {
+        // Slots of a slice: the sinks' blocks first, per_sink items each.
+        map_block(blockIdx.x, p.slots, p.B * p.Hkv, false, bk, slot);
+        const int sink_slots = p.sink_blocks * p.per_sink;
+        const bool sink = slot < sink_slots;
+        per = sink ? p.per_sink : p.per_block;
+        const int i0 = sink ? slot : slot - sink_slots;
+        kb = (sink ? 0 : p.sink_blocks) + i0 / per;
+        c = i0 % per;
+        b = bk / p.Hkv;
+        hk = bk - b * p.Hkv;
+        G = p.H / p.Hkv;
+        kl = window_keys(p, b);
+    }
+};
+// dV and dK of key kj (row kj - k0 of the block), channels d .. d + 3: the gradients,
+// or one item's unscaled sums. live: the key takes part.
 template <int D, typename T>
-GONN_DEV void window_dkdv_plain(const WindowParams& p, int b, int hk, const T* krow, const T* vrow,
-                                const BlockSteps& bs, int BQ, int s0, int s1, const Band& band,
-                                int kl, int kw, int kj, f32x16* acc) {
-    constexpr int NDT = D / 32;
-    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31, G = p.H / p.Hkv;
-    for (int t = 0; t < 2 * NDT; t++) acc[t] = f32x16{};
+GONN_DEV void write_dkdv(const WindowParams& p, const DkdvItem& it, int BK, int kj, int k0, int d,
+                         f32x4 dv, f32x4 dk, bool live) {
+    if (!live) dv = dk = f32x4{};
+    if (it.per > 1) {
+        float* part = p.part + (((size_t)it.bk * p.slots + it.slot) * 2 * BK + kj - k0) * D + d;
+        *(f32x4*)part = dv;
+        *(f32x4*)(part + (size_t)BK * D) = dk;
+    } else {
+        const size_t x = ((size_t)it.bk * p.Sk + kj) * D + d;
+        store4<T>((T*)p.dv + x, dv);
+        store4<T>((T*)p.dk + x, dk * p.scale);
+    }
+}
+
+// dV and dK of a wave's 32 keys over steps [s0, s1), plain fp32 products, 32 channels
+// at a time.
+template <int D, typename T>
+GONN_DEV void window_dkdv_plain(const WindowParams& p, const DkdvItem& it, const BlockSteps& bs,
+                                int BK, int BQ, int s0, int s1, const Band& band, int kw) {
+    const int lane = threadIdx.x & 63, g = lane >> 5, ln = lane & 31, kj = kw + ln;
+    const size_t kr = ((size_t)it.bk * p.Sk + (kj < p.Sk ? kj : p.Sk - 1)) * D;
+    const T *krow = (const T*)p.k + kr, *vrow = (const T*)p.v + kr;
 #pragma unroll 1
-    for (int st = s0; st < s1; st++) {
-        const size_t base = ((size_t)b * p.H + hk * G + st / bs.nst) * p.Sq;
+    for (int t = 0; t < D / 32; t++) {
+        f32x16 dv = f32x16{}, dk = f32x16{};
 #pragma unroll 1
-        for (int off = 0; off < BQ; off += 32) {
-            const int q0 = (bs.st0 + st % bs.nst) * BQ + off;
-            if (q0 >= p.Sq || !band.any(q0, q0 + 31, kw, kw + 31)) continue;
-            const size_t qr = (base + (q0 + ln < p.Sq ? q0 + ln : p.Sq - 1)) * D;
-            f32x16 s, dp;
-            plain_products<D>((const T*)p.q + qr, krow, (const T*)p.dO + qr, vrow, g, s, dp);
-            for (int r = 0; r < 16; r++) {
-                const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3), qc = q < p.Sq ? q : p.Sq - 1;
-                const bool on = q < p.Sq && kj < kl && band.sees(q, kj);
-                const float pv =
-                    fast_exp2(__builtin_fmaf(s[r], p.scale_log2, -lse_log2(p.lse_in[base + qc])));
-                s[r] = on ? pv : 0.f;
-                dp[r] = on ? pv * (dp[r] - p.delta[base + qc]) : 0.f;
-            }
+        for (int st = s0; st < s1; st++) {
+            const size_t bh = (size_t)it.b * p.H + it.hk * it.G + st / bs.nst, base = bh * p.Sq;
 #pragma unroll 1
-            for (int x = 0; x < 32; x++) {
-                const int r = x >> 1, h = x & 1, q = q0 + 8 * (r >> 2) + 4 * h + (r & 3);
-                const float wp = weight_of(s, r, h, g), wd = weight_of(dp, r, h, g);
-                if (q >= p.Sq) continue;  // uniform
-                const bool on = kj < kl && band.sees(q, kj);
-                add_row<D>(acc, wp, (const T*)p.dO + (base + q) * D, g, on);
-                add_row<D>(acc + NDT, wd, (const T*)p.q + (base + q) * D, g, on);
+            for (int off = 0; off < BQ; off += 32) {
+                const int q0 = (bs.st0 + st % bs.nst) * BQ + off;
+                if (q0 >= p.Sq || !band.any(q0, q0 + 31, kw, kw + 31)) continue;
+                const size_t qr = (base + (q0 + ln < p.Sq ? q0 + ln : p.Sq - 1)) * D;
+                f32x16 s, dp;
+                plain_products<D>((const T*)p.q + qr, krow, (const T*)p.dO + qr, vrow, g, s, dp);
+                for (int r = 0; r < 16; r++) {
+                    const int q = q0 + 8 * (r >> 2) + 4 * g + (r & 3), qc = q < p.Sq ? q : p.Sq - 1;
+                    const bool on = q < p.Sq && kj < it.kl && band.sees(q, kj);
+                    const float pv = fast_exp2(__builtin_fmaf(s[r], p.scale_log2, -p.lse2[bh * p.Sp + qc]));
+                    s[r] = on ? pv : 0.f;
+                    dp[r] = on ? pv * (dp[r] - p.delta[bh * p.Sp + qc]) : 0.f;
+                }
+#pragma unroll 1
+                for (int x = 0; x < 32; x++) {
+                    const int r = x >> 1, h = x & 1, q = q0 + 8 * (r >> 2) + 4 * h + (r & 3);
+                    const float wp = weight_of(s, r, h, g), wd = weight_of(dp, r, h, g);
+                    if (q >= p.Sq) continue;  // uniform
+                    const bool on = kj < it.kl && band.sees(q, kj);
+                    add_row32(dv, wp, (const T*)p.dO + (base + q) * D + 32 * t, g, on);
+                    add_row32(dk, wd, (const T*)p.q + (base + q) * D + 32 * t, g, on);
+                }
             }
         }
+        if (kj < p.Sk)
+            for (int rq = 0; rq < 4; rq++) {
+                f32x4 x, y;
+                for (int i = 0; i < 4; i++) {
+                    x[i] = dv[rq * 4 + i];
+                    y[i] = dk[rq * 4 + i];
+                }
+                write_dkdv<D, T>(p, it, BK, kj, kw / BK * BK, 32 * t + 8 * rq + 4 * g, x, y, kj < it.kl);
+            }
     }
 }
 
@@ -248,20 +310,14 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = wave % WB, ws = wave / WB, g = lane >> 5, ln = lane & 31;
-    // Slot of the slice's items: the sinks' blocks first, per_sink each.
-    int bk, slot;
-    map_block(blockIdx.x, p.slots, p.B * p.Hkv, false, bk, slot);
-    const int sink_slots = p.sink_blocks * p.per_sink;
-    const bool sink = slot < sink_slots;
-    const int per = sink ? p.per_sink : p.per_block;
-    const int i0 = sink ? slot : slot - sink_slots;
-    const int kb = (sink ? 0 : p.sink_blocks) + i0 / per, c = i0 % per;
-    const int b = bk / p.Hkv, hk = bk - b * p.Hkv, G = p.H / p.Hkv, kl = window_keys(p, b);
-    const int k0 = kb * BK, kw = k0 + wb * 32, kj = kw + ln;
+    DkdvItem it;
+    it.init(p);
+    const int bk = it.bk, b = it.b, hk = it.hk, G = it.G, kl = it.kl, per = it.per;
+    const int k0 = it.kb * BK, kw = k0 + wb * 32, kj = kw + ln;
     const Band band{p.window, p.sinks};
     BlockSteps bs;
     bs.init(k0, BK, BQ, p.Sq, kl, band);
-    const int s0 = c * p.chunk;
+    const int s0 = it.c * p.chunk;
     int s1 = bs.nst * G;
     s1 = per > 1 && s1 - s0 > p.chunk ? s0 + p.chunk : s1;
     if (per > 1 && s0 >= s1) return;  // no such item: nothing is read from its slot
@@ -270,13 +326,13 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     in.init(tid);
     float rl = 0.f, rd = 0.f;
     auto gload = [&](int st) {
-        const size_t base = ((size_t)b * p.H + hk * G + st / bs.nst) * p.Sq;
+        const size_t bh = (size_t)b * p.H + hk * G + st / bs.nst;
         const int q0 = (bs.st0 + st % bs.nst) * BQ;
-        in.load((const T*)p.q + base * D, (const T*)p.dO + base * D, q0, p.Sq);
+        in.load((const T*)p.q + bh * p.Sq * D, (const T*)p.dO + bh * p.Sq * D, q0, p.Sq);
         if (tid < BQ) {
             const int q = q0 + tid;
-            rl = q < p.Sq ? lse_log2(p.lse_in[base + q]) : INFINITY;
-            rd = q < p.Sq ? p.delta[base + q] : 0.f;
+            rl = q < p.Sp ? p.lse2[bh * p.Sp + q] : INFINITY;
+            rd = q < p.Sp ? p.delta[bh * p.Sp + q] : 0.f;
         }
     };
     auto sstore = [&](int buf) {
@@ -356,28 +412,20 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
                 else bad |= nonfinite(acc[t][r]);
             }
         if constexpr (NP == 3) bad = chk.plain();
-        if (__builtin_amdgcn_ballot_w64(bad && kj < kl))
-            window_dkdv_plain<D>(p, b, hk, krow, vrow, bs, BQ, s0, s1, band, kl, kw, kj, acc);
+        if (__builtin_amdgcn_ballot_w64(bad && kj < kl)) {
+            window_dkdv_plain<D, T>(p, it, bs, BK, BQ, s0, s1, band, kw);
+            return;
+        }
     }
     if (kj >= p.Sk) return;
-    const bool live = kj < kl;
-    // Partials hold the unscaled sums.
-    float* part = per > 1 ? p.part + (((size_t)bk * p.slots + slot) * 2 * BK + kj - k0) * D : nullptr;
     for (int t = 0; t < NDT; t++)
         for (int rq = 0; rq < 4; rq++) {
-            f32x4 dv, dk;
+            f32x4 x, y;
             for (int i = 0; i < 4; i++) {
-                dv[i] = live ? acc[t][rq * 4 + i] : 0.f;
-                dk[i] = live ? acc[NDT + t][rq * 4 + i] : 0.f;
+                x[i] = acc[t][rq * 4 + i];
+                y[i] = acc[NDT + t][rq * 4 + i];
             }
-            const int d = t * 32 + rq * 8 + g * 4;
-            if (part) {
-                *(f32x4*)(part + d) = dv;
-                *(f32x4*)(part + (size_t)BK * D + d) = dk;
-            } else {
-                store4<T>((T*)p.dv + kr + d, dv);
-                store4<T>((T*)p.dk + kr + d, dk * p.scale);
-            }
+            write_dkdv<D, T>(p, it, BK, kj, k0, t * 32 + rq * 8 + g * 4, x, y, kj < kl);
         }
 }
 

@@ -140,12 +140,18 @@ struct WindowParams {
     int window, sinks;
     float scale;       // signed
     float scale_log2;  // scale * log2(e)
+    // The same with the sign apart, which kernels that mask scores with -inf ahead of
+    // the scaling fold into an operand: |scale| log2(e) and sign(scale); log2(e) and 0
+    // for a scale of 0.
+    float c2, sign;
     const int* kv_len;  // [B] or null (all Sk)
-    // Backward: the saved o and lse, dO, the gradients; delta (B*H, Sq) is
-    // written by the dQ kernel and read by the dK/dV kernel after it.
+    // Backward: the saved o and lse, dO, the gradients; lse2 (LSE log2(e), +inf for
+    // rows without keys and for pad rows) and delta (0 on pad rows), both (B*H, Sp),
+    // are written by the dQ kernel and read by the dK/dV kernel after it.
     const void *o_in, *dO;
     const float* lse_in;
-    float* delta;
+    float *lse2, *delta;
+    int Sp;  // Sq rounded up to 64
     void *dq, *dk, *dv;
     // dK/dV work items (attn_window_bwd.hip): the (head, query stage) steps of
     // a key block are cut in chunks of `chunk`; blocks of more than one leave
