@@ -429,6 +429,362 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
         }
 }
 
+// ---------------------------------------------------------------------------
+// bf16 dK/dV of large grids: 128 keys per workgroup (32 per wave, K and V in
+// registers), query tiles of 64 in four-slot LDS rings filled straight from memory,
+// one wave per SIMD, in the hand-ordered three-stage pipeline of attn_bwd.hip. Step
+// i issues, without dependences between them,
+//   MFMA  S(i+1) = Q K^T, dP(i+1) = dO V^T
+//   VALU  P(i) = exp2(S c2 - LSE log2e), dS(i) = P (dP - delta), packed to bf16
+//   MFMA  dV^T += dO^T P(i-1), dK^T += Q^T dS(i-1)
+// over the query heads and tiles of its item in turn. Slot e issues the LDS read of
+// MFMA e + 3, MFMA e, a tile load and the VALU work mapped to it. Masked scores are
+// set to -inf between steps, on tiles that cross the window's or the causal edge. S
+// and dP have VGPR accumulators and K and V lie in AGPRs (inline asm, whose wait
+// states the kernel provides itself: three s_nop 7 that the accumulators pass
+// through behind each step's last such MFMA).
+// ---------------------------------------------------------------------------
+GONN_DEV void mfma_vacc0(f32x16& d, bf16x8 a, bf16x8 b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(b));
+}
+GONN_DEV void mfma_vacc(f32x16& d, bf16x8 a, bf16x8 b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(b));
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 1) void window_dkdv_pipe_kernel(WindowParams p) {
+    constexpr int BK = 128, BQ = 64, NKS = D / 16, NDT = D / 32;
+    constexpr int RTILE = BQ * D;  // elements of a Q or dO tile
+    constexpr uint32_t RTB = RTILE * 2;
+    constexpr int NRI = RTILE / 8 / 256, NSLOT = 4;
+    __shared__ __attribute__((aligned(16))) bf16 sQ[NSLOT * RTILE];
+    __shared__ __attribute__((aligned(16))) bf16 sdO[NSLOT * RTILE];
+    __shared__ __attribute__((aligned(16))) float sLD[2][2 * BQ];  // lse2, then delta
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 5, ln = lane & 31;
+    DkdvItem it;
+    it.init(p);
+    const int k0 = it.kb * BK, kw = k0 + wave * 32, kj = kw + ln, kl = it.kl;
+    const Band band{p.window, p.sinks};
+    BlockSteps bs;
+    bs.init(k0, BK, BQ, p.Sq, kl, band);
+    const int s0 = it.c * p.chunk;
+    int nq = bs.nst * it.G - s0;
+    nq = it.per > 1 && nq > p.chunk ? p.chunk : nq;
+    if (nq <= 0) {  // no such item, or no query sees the block
+        if (it.per > 1) return;
+        for (int i = tid; i < BK * D / 4; i += 256) {
+            const int r = i / (D / 4);
+            if (k0 + r < p.Sk)
+                write_dkdv<D, bf16>(p, it, BK, k0 + r, k0, i % (D / 4) * 4, f32x4{}, f32x4{}, false);
+        }
+        return;
+    }
+
+    bf16x8 kf[NKS], vf[NKS];
+    {
+        const size_t kr = ((size_t)it.bk * p.Sk + (kj < p.Sk ? kj : p.Sk - 1)) * D;
+        const bf16 *krow = (const bf16*)p.k + kr + g * 8, *vrow = (const bf16*)p.v + kr + g * 8;
+        // The scale's sign goes into K here, so that -inf masks stay -inf.
+        const uint32_t flip = p.sign < 0.f ? 0x80008000u : 0u, keep = p.sign != 0.f ? ~0u : 0u;
+        for (int ks = 0; ks < NKS; ks++) {
+            u32x4 a = u32x4{}, c = u32x4{};
+            if (kj < kl) {
+                a = *(const u32x4*)(krow + ks * 16);
+                c = *(const u32x4*)(vrow + ks * 16);
+            }
+            for (int e = 0; e < 4; e++) a[e] = (a[e] ^ flip) & keep;
+            kf[ks] = __builtin_bit_cast(bf16x8, a);
+            vf[ks] = __builtin_bit_cast(bf16x8, c);
+        }
+    }
+    for (int ks = 0; ks < NKS; ks++) {  // into AGPRs, then wait states
+        asm volatile("s_nop 4" : "+a"(kf[ks]));
+        asm volatile("s_nop 4" : "+a"(vf[ks]));
+    }
+    asm volatile("s_nop 7");
+
+    // Step s of the item: query tile qt of head hh. One cursor per pipeline stage.
+    struct Cursor {
+        int hh, qt;
+    };
+    const int st0 = bs.st0, stE = bs.st0 + bs.nst;
+    auto next = [&](Cursor c) {
+        c.qt++;
+        if (c.qt == stE) {
+            c.qt = st0;
+            c.hh++;
+        }
+        return c;
+    };
+    const int Sq = p.Sq, Sp = p.Sp;
+    const size_t h0 = (size_t)it.b * p.H + it.hk * it.G;
+    const bf16* Qg = (const bf16*)p.q + h0 * Sq * D;
+    const bf16* dOg = (const bf16*)p.dO + h0 * Sq * D;
+    // One resource over the key head's query heads: rows past a head's last are the
+    // next head's, or zeros, and lse2 = +inf gives them no weight.
+    const uint32_t bytes = (uint32_t)it.G * Sq * D * 2, lbytes = (uint32_t)it.G * Sp * 4;
+    const brsrc rq = make_rsrc(Qg, bytes), rdo = make_rsrc(dOg, bytes);
+    const brsrc rl = make_rsrc(p.lse2 + h0 * Sp, lbytes), rd = make_rsrc(p.delta + h0 * Sp, lbytes);
+    uint32_t roff[NRI];
+    for (int i = 0; i < NRI; i++) {
+        int r, c;
+        slab_chunk(i * 256 + tid, BQ, r, c);
+        roff[i] = (uint32_t)((r * D + c * 8) * 2);
+    }
+    const uint32_t lq = lds_addr(sQ) + wave * 1024, ldo = lds_addr(sdO) + wave * 1024;
+    auto dma_row = [&](uint32_t so, int slot, int j, uint32_t on) {
+        const int i = j % NRI;
+        dma16_if(j < NRI ? rq : rdo, (j < NRI ? lq : ldo) + slot * RTB + i * 4096, roff[i], so, on);
+    };
+    auto row_off = [&](Cursor c) { return (uint32_t)((c.hh * Sq + c.qt * BQ) * D) * 2u; };
+    auto dma_ld = [&](Cursor c, int slot) {
+        if (wave == 0) {
+            const uint32_t dl = lds_addr(sLD) + slot * 2 * BQ * 4, so = (uint32_t)(c.hh * Sp + c.qt * BQ) * 4u;
+            if (lane < 16) dma16(rl, dl, (lane & 15) * 16, so);
+            else if (lane < 32) dma16(rd, dl, (lane & 15) * 16, so);
+        }
+    };
+
+    // Operand reads (bytes from a slot's start), as in attn_bwd.hip.
+    const int hs = slab_swz(ln);
+    const uint32_t ra0 = (uint32_t)(ln * 64 + ((0 + g) ^ hs) * 16);
+    const uint32_t ra1 = (uint32_t)(ln * 64 + ((2 + g) ^ hs) * 16);
+    const int s16 = lane & 15;
+    const int tcx = 2 * ((ln >> 4) & 1) + ((s16 >> 1) & 1);
+    const uint32_t ta0 = (uint32_t)((4 * g + (s16 >> 2)) * 64 + (tcx ^ g) * 16 + 8 * (s16 & 1));
+    const uint32_t ta1 =
+        (uint32_t)((8 + 4 * g + (s16 >> 2)) * 64 + (tcx ^ (2 + g)) * 16 + 8 * (s16 & 1));
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    typedef __attribute__((address_space(3))) char lds_char;
+    lds_char* const tQ = (lds_char*)sQ;
+    lds_char* const tdO = (lds_char*)sdO;
+    const char* cQ = (const char*)sQ;
+    const char* cdO = (const char*)sdO;
+    auto rowa = [&](int kk, int mt) {
+        return (uint32_t)(((kk >> 1) * BQ + mt * 32) * 64) + ((kk & 1) ? ra1 : ra0);
+    };
+
+    f32x16 dvacc[NDT], dkacc[NDT];
+    for (int t = 0; t < NDT; t++) dvacc[t] = dkacc[t] = f32x16{};
+    const float c2 = p.c2;
+    u32x4 pp[4], pd[4];  // P and dS of the tile dV/dK consume next
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+    // Scores of query tile qt that this lane's key is not seen by, to -inf.
+    auto mask = [&](int qt, f32x16* s) {
+        const int q0 = qt * BQ;
+        if (kw + 32 <= kl && band.all(q0, q0 + BQ - 1, kw, kw + 31)) return;  // wave-uniform
+        // Query 8 (r / 4) + r % 4 + 32 mt of the lane group: from lo on, and below hi.
+        const int lo = kj < kl ? kj - q0 - 4 * g : BQ;
+        const int hi = kj < p.sinks ? BQ : lo + p.window;
+        for (int mt = 0; mt < 2; mt++)
+            for (int r = 0; r < 16; r++) {
+                const int c = mt * 32 + 8 * (r >> 2) + (r & 3);
+                s[mt][r] = c < lo || c >= hi ? -INFINITY : s[mt][r];
+            }
+    };
+    // One pipeline step. sA <- S(i+1), dA <- dP(i+1); sB, dB = S(i), dP(i). c1, c2q:
+    // the cursors of tiles i + 1 and i + 2.
+    auto step = [&](auto ha_tag, auto hb_tag, auto hc_tag, int i, Cursor c1, Cursor c2q, f32x16* sA,
+                    f32x16* dA, f32x16* sB, f32x16* dB) __attribute__((always_inline)) {
+        constexpr bool HA = decltype(ha_tag)::value;  // S/dP of tile i+1
+        constexpr bool HB = decltype(hb_tag)::value;  // P/dS of tile i
+        constexpr bool HC = decltype(hc_tag)::value;  // dV/dK of tile i-1
+        const uint32_t dr = HA && i + 2 < nq;
+        if (HA) dma_ld(c1, (i + 1) & 1);
+        const uint32_t so2 = row_off(c2q);
+        const uint32_t rsl = (uint32_t)((i + 1) & 3) * RTB;  // tile i+1 (S, dP)
+        const uint32_t tsl = (uint32_t)((i + 3) & 3) * RTB;  // tile i-1 (dV, dK)
+        const uint32_t nsl = (uint32_t)((i + 2) & 3);        // slot of tile i+2
+        const int lsl = i & 1;
+
+        constexpr int HCn = HC ? 2 * NDT : 0, HAn = HA ? NKS : 0;
+        constexpr int GW = HCn + HAn;  // MFMAs per 16-query k-step group
+        constexpr int NM = 4 * GW, LA = 3, NO = 4;
+        constexpr int NDMA = 2 * NRI, SPAN = 16 < NM ? 16 : NM;
+        constexpr int DS = SPAN / NDMA > 0 ? SPAN / NDMA : 1;
+        bf16x8 opr[NO];
+        auto fetch = [&](auto E) {
+            constexpr int e = decltype(E)::value, ks = e / GW, w = e % GW;
+            if constexpr (w < HCn) {
+                constexpr int t = w % NDT;
+                lds_char* const base = (w < NDT ? tdO : tQ) + tsl + (t * BQ + 16 * ks) * 64;
+                const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + ta0));
+                const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(base + ta1));
+                const s4 b8[2] = {lo, hi};
+                opr[e % NO] = __builtin_bit_cast(bf16x8, b8);
+            } else {
+                constexpr int u = w - HCn, kk = ks * (NKS / 4) + u / 4, mt = u & 1;
+                const char* base = ((u & 2) ? cdO : cQ) + rsl;
+                opr[e % NO] = *(const bf16x8*)(base + rowa(kk, mt));
+            }
+        };
+        auto issue = [&](auto E) {
+            constexpr int e = decltype(E)::value, ks = e / GW, w = e % GW;
+            if constexpr (w < HCn) {
+                constexpr int t = w % NDT;
+                if constexpr (w < NDT)
+                    dvacc[t] = mfma_bf16(opr[e % NO], __builtin_bit_cast(bf16x8, pp[ks]), dvacc[t]);
+                else
+                    dkacc[t] = mfma_bf16(opr[e % NO], __builtin_bit_cast(bf16x8, pd[ks]), dkacc[t]);
+            } else {
+                constexpr int u = w - HCn, kk = ks * (NKS / 4) + u / 4, mt = u & 1;
+                f32x16& acc = (u & 2) ? dA[mt] : sA[mt];
+                const bf16x8& b = (u & 2) ? vf[kk] : kf[kk];
+                if constexpr (kk == 0) mfma_vacc0(acc, opr[e % NO], b);
+                else mfma_vacc(acc, opr[e % NO], b);
+            }
+        };
+        // VALU of tile i in 8 groups (registers 4 j4 .. of sB/dB[mt]) of five
+        // micro-ops; group k fills words of k-step k / 2 behind its dV/dK MFMAs.
+        f32x4 uL[8], uD[8];
+        float ue[8][4];
+        auto ub = [](int k, int st) {
+            int b0 = (k >> 1) * GW + (HCn ? HCn - 1 : 0) + 2 * (k & 1);
+            const int off[5] = {-5, -3, -2, 0, 1};
+            const int s = b0 + off[st];
+            return s < 0 ? 0 : s;
+        };
+        auto uop = [&](auto K, auto ST) {
+            constexpr int k = decltype(K)::value, st = decltype(ST)::value;
+            constexpr int mt = k >> 2, j4 = k & 3, ks = k >> 1, w0 = (j4 & 1) * 2;
+            if constexpr (st == 0) {
+                uL[k] = *(const f32x4*)&sLD[lsl][mt * 32 + 8 * j4 + 4 * g];
+                uD[k] = *(const f32x4*)&sLD[lsl][BQ + mt * 32 + 8 * j4 + 4 * g];
+            } else if constexpr (st <= 2) {
+                constexpr int e0 = (st - 1) * 2;
+                for (int e = e0; e < e0 + 2; e++) {
+                    ue[k][e] = fast_exp2(__builtin_fmaf(sB[mt][4 * j4 + e], c2, -uL[k][e]));
+                    pin(ue[k][e]);
+                }
+            } else {
+                constexpr int e0 = (st - 3) * 2;
+                const float d0 = ue[k][e0] * (dB[mt][4 * j4 + e0] - uD[k][e0]);
+                const float d1 = ue[k][e0 + 1] * (dB[mt][4 * j4 + e0 + 1] - uD[k][e0 + 1]);
+                const bf16x2 pr = {to_bf16(ue[k][e0]), to_bf16(ue[k][e0 + 1])};
+                const bf16x2 dr2 = {to_bf16(d0), to_bf16(d1)};
+                pp[ks][w0 + e0 / 2] = __builtin_bit_cast(uint32_t, pr);
+                pd[ks][w0 + e0 / 2] = __builtin_bit_cast(uint32_t, dr2);
+                pin(pp[ks][w0 + e0 / 2]);
+                pin(pd[ks][w0 + e0 / 2]);
+            }
+        };
+        auto uops_at = [&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (HB) {
+                static_for<5>([&](auto ST) {
+                    static_for<8>([&](auto K) {
+                        constexpr int at = ub(decltype(K)::value, decltype(ST)::value);
+                        if constexpr (e < NM ? at == e : at >= NM) uop(K, ST);
+                    });
+                });
+            }
+        };
+        static_for<LA>([&](auto E) {
+            if constexpr (decltype(E)::value < NM) fetch(E);
+        });
+        static_for<NM>([&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (e + LA < NM) fetch(std::integral_constant<int, e + LA>{});
+            issue(E);
+            if constexpr (e >= 1 && (e - 1) % DS == 0 && (e - 1) / DS < NDMA)
+                dma_row(so2, nsl, (e - 1) / DS, dr);
+            uops_at(E);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        static_for<NDMA>([&](auto Dd) {
+            constexpr int d = decltype(Dd)::value;
+            if constexpr (NM == 0 || 1 + d * DS >= NM) dma_row(so2, nsl, d, dr);
+        });
+        uops_at(std::integral_constant<int, NM>{});
+        if constexpr (HA)
+            asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
+                         : "+v"(sA[0]), "+v"(sA[1]), "+v"(dA[0]), "+v"(dA[1]));
+        GONN_VMCNT(0);
+        __syncthreads();
+        if constexpr (HA) mask(c1.qt, sA);
+    };
+    using Yes = std::integral_constant<bool, true>;
+    using No = std::integral_constant<bool, false>;
+
+    // Prologue: tiles 0, 1 and L/D of tile 0; S/dP of tile 0.
+    Cursor c0{s0 / bs.nst, st0 + s0 % bs.nst};
+    Cursor ca = next(c0), cb = next(ca);
+    for (int j = 0; j < 2 * NRI; j++) dma_row(row_off(c0), 0, j, 1);
+    for (int j = 0; j < 2 * NRI; j++) dma_row(row_off(ca), 1, j, nq > 1);
+    dma_ld(c0, 0);
+    GONN_VMCNT(0);
+    __syncthreads();
+    f32x16 sX[2], dX[2], sY[2], dY[2];
+    for (int kk = 0; kk < NKS; kk++)
+        for (int mt = 0; mt < 2; mt++) {
+            const bf16x8 aq = *(const bf16x8*)(cQ + rowa(kk, mt));
+            const bf16x8 ad = *(const bf16x8*)(cdO + rowa(kk, mt));
+            if (kk == 0) {
+                mfma_vacc0(sX[mt], aq, kf[kk]);
+                mfma_vacc0(dX[mt], ad, vf[kk]);
+            } else {
+                mfma_vacc(sX[mt], aq, kf[kk]);
+                mfma_vacc(dX[mt], ad, vf[kk]);
+            }
+        }
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(sX[0]), "+v"(sX[1]), "+v"(dX[0]), "+v"(dX[1]));
+    mask(c0.qt, sX);
+
+    // Steps 0 .. nq, the full ones in pairs (see attn_bwd.hip).
+    auto advance = [&] {
+        ca = cb;
+        cb = next(cb);
+    };
+    if (nq == 1) {
+        step(No{}, Yes{}, No{}, 0, ca, cb, sY, dY, sX, dX);
+        step(No{}, No{}, Yes{}, 1, ca, cb, sX, dX, sY, dY);
+    } else {
+        step(Yes{}, Yes{}, No{}, 0, ca, cb, sY, dY, sX, dX);
+        advance();
+        int i = 1;
+        if ((nq - 2) & 1) {
+            step(Yes{}, Yes{}, Yes{}, 1, ca, cb, sX, dX, sY, dY);
+            advance();
+            for (int mt = 0; mt < 2; mt++) {
+                sY[mt] = sX[mt];
+                dY[mt] = dX[mt];
+            }
+            i = 2;
+        }
+        for (; i < nq - 1; i += 2) {
+            step(Yes{}, Yes{}, Yes{}, i, ca, cb, sX, dX, sY, dY);
+            advance();
+            step(Yes{}, Yes{}, Yes{}, i + 1, ca, cb, sY, dY, sX, dX);
+            advance();
+        }
+        step(No{}, Yes{}, Yes{}, nq - 1, ca, cb, sX, dX, sY, dY);
+        step(No{}, No{}, Yes{}, nq, ca, cb, sY, dY, sX, dX);
+    }
+
+    bool bad = false;
+    for (int t = 0; t < NDT; t++)
+        for (int r = 0; r < 16; r++) bad |= nonfinite(dvacc[t][r]) || nonfinite(dkacc[t][r]);
+    if (__builtin_amdgcn_ballot_w64(bad && kj < kl)) {
+        window_dkdv_plain<D, bf16>(p, it, bs, BK, BQ, s0, s0 + nq, band, kw);
+        return;
+    }
+    if (kj >= p.Sk) return;
+    for (int t = 0; t < NDT; t++)
+        for (int rq4 = 0; rq4 < 4; rq4++) {
+            f32x4 x, y;
+            for (int k = 0; k < 4; k++) {
+                x[k] = dvacc[t][rq4 * 4 + k];
+                y[k] = dkacc[t][rq4 * 4 + k];
+            }
+            write_dkdv<D, bf16>(p, it, BK, kj, k0, t * 32 + rq4 * 8 + g * 4, x, y, kj < kl);
+        }
+}
+
 // dK and dV of the blocks of several items: their partials in order. Four
 // elements a thread; blocks [0, nb) of each slice.
 template <int D, typename T>
@@ -466,18 +822,25 @@ namespace {
 struct DkdvShape {
     int BK, BQ;
 };
-DkdvShape dkdv_shape(const WindowParams& p, int is_bf16) {
+DkdvShape dkdv_shape(const WindowParams& p, int D, int is_bf16) {
     const long long cus = device_cus();
     const long long b128 = (long long)((p.Sk + 127) / 128) * p.B * p.Hkv;
-    if (b128 >= cus && is_bf16) return {128, 32};
+    // The 128-key kernel reads a key head's queries with 32-bit offsets.
+    const bool near = (double)(p.H / p.Hkv) * p.Sp * D * 2 < 4.0e9;
+    if (b128 >= cus && is_bf16 && near) return {128, 64};
     return {64, 64};
 }
 
-template <int D, typename T, int WB, int NBUF, int OCC>
-void run_dkdv(const WindowParams& p, hipStream_t s) {
+template <int D, typename T>
+void run_dkdv(const WindowParams& p, int BK, int BQ, hipStream_t s) {
     const unsigned grid = (unsigned)p.slots * (unsigned)(p.B * p.Hkv);
-    window_dkdv_kernel<D, T, WB, NBUF, OCC><<<grid, 256, 0, s>>>(p);
-    const int BK = WB * 32, BQ = 4 / WB * 32, nkb = (p.Sk + BK - 1) / BK;
+    if constexpr (sizeof(T) == 2) {
+        if (BK == 128) window_dkdv_pipe_kernel<D><<<grid, 256, 0, s>>>(p);
+        else window_dkdv_kernel<D, T, 2, 2, 1><<<grid, 256, 0, s>>>(p);
+    } else {
+        window_dkdv_kernel<D, T, 2, 1, 1><<<grid, 256, 0, s>>>(p);
+    }
+    const int nkb = (p.Sk + BK - 1) / BK;
     const int nb = p.per_block > 1 ? nkb : (p.per_sink > 1 ? p.sink_blocks : 0);
     if (!nb) return;
     const size_t n = (size_t)p.B * p.Hkv * nb * BK * 2 * (D / 4);
@@ -489,22 +852,20 @@ void run_window_bwd(const WindowParams& p, hipStream_t s) {
     const long long cus = device_cus(), BH = (long long)p.B * p.H;
     const long long b128 = (long long)((p.Sq + 127) / 128) * BH;
     const unsigned g128 = (unsigned)b128, g64 = (unsigned)((p.Sq + 63) / 64 * BH);
-    const DkdvShape sh = dkdv_shape(p, sizeof(T) == 2);
+    const DkdvShape sh = dkdv_shape(p, D, sizeof(T) == 2);
     if constexpr (sizeof(T) == 2) {
         if (b128 >= 2 * cus) window_dq_kernel<D, T, 4, 2, 2><<<g128, 256, 0, s>>>(p);
         else window_dq_kernel<D, T, 2, 2, 1><<<g64, 256, 0, s>>>(p);
-        if (sh.BK == 128) run_dkdv<D, T, 4, 2, 1>(p, s);
-        else run_dkdv<D, T, 2, 2, 1>(p, s);
     } else {
         window_dq_kernel<D, T, 2, 1, 1><<<g64, 256, 0, s>>>(p);
-        run_dkdv<D, T, 2, 1, 1>(p, s);
     }
+    run_dkdv<D, T>(p, sh.BK, sh.BQ, s);
 }
 
 }  // namespace
 
 size_t plan_window_bwd(WindowParams& p, int D, int is_bf16) {
-    const DkdvShape sh = dkdv_shape(p, is_bf16);
+    const DkdvShape sh = dkdv_shape(p, D, is_bf16);
     const long long slices = (long long)p.B * p.Hkv, G = p.H / p.Hkv, want = 2 * device_cus();
     const int nkb = (p.Sk + sh.BK - 1) / sh.BK;
     const long long all = G * ((p.Sq + sh.BQ - 1) / sh.BQ);

@@ -103,6 +103,13 @@ def test_results_are_waited_for_on_every_path(name, tmp_path):
     assert "v_mfma_f32_32x32x16_bf16" in text
     bad = scan(text)
     assert not bad, (len(bad), bad[:3])
+    if name == "attn_window_bwd.hip":  # its inline MFMAs: the rules of test_asm_hazards
+        from tests.test_asm_hazards import _scan
+        fns = [f for f in re.split(r"\n(?=[A-Za-z_][\w.$]*:)", text) if f.startswith("_ZN4gonn23window_dkdv_pipe_kernel")]
+        assert len(fns) == 2
+        for f in fns:
+            broken, first = _scan(f.split(".Lfunc_end")[0].split("\n"))
+            assert first is not None and not broken, (len(broken), broken[:3])
 
 
 def test_the_scan_follows_branches():

@@ -25,6 +25,10 @@ CASES = [
     (4, 16, 4, 256, 256, 64, 40, 5, None),           # 64-row blocks
     (16, 16, 16, 200, 200, 64, 50, 3, (200,) * 15 + (77,)),  # 128-row blocks
     (16, 16, 16, 150, 150, 128, 64, 0, None),
+    # Large grids with shared key heads: items over several query heads.
+    (8, 64, 32, 300, 300, 64, 40, 5, (300, 1, 64, 128, 129, 200, 299, 0)),
+    (4, 64, 32, 260, 300, 128, 100, 140, None),
+    (2, 32, 16, 1100, 1100, 64, 128, 4, None),
 ]
 
 
@@ -110,10 +114,12 @@ def test_scales(scale, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("bad", [math.inf, math.nan], ids=["inf", "nan"])
-@pytest.mark.parametrize("S", [70, 330])
-def test_bad_values_reach_only_those_that_see_them(dtype, bad, S):
+@pytest.mark.parametrize("S,big", [(70, False), (330, False), (100, True)])
+def test_bad_values_reach_only_those_that_see_them(dtype, bad, S, big):
     from gonn_amd import hip
     c = (2, 4, 2, S, S, 64, 20, 3, (S, S - 30))
+    if big:  # the kernels of large grids
+        c = (32, 16, 8, S, S, 64, 20, 3, (S, S - 30) * 16)
     window, sinks, kv = c[6:]
     scale = 1.0 / 8
     for where in ("v", "k", "q", "dO", "pad"):
