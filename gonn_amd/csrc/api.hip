@@ -435,12 +435,13 @@ int check_window_bwd(const gonn_attn_window_bwd_args* a, gonn::WindowParams* p) 
 size_t window_bwd_ws(gonn::WindowParams& p, int D, int is_bf16, void* ws) {
     p.Sp = (int)round_up((size_t)p.Sq, 64);
     const size_t rows = round_up((size_t)p.B * p.H * p.Sp * sizeof(float), 256);
-    const size_t part = gonn::plan_window_bwd(p, D, is_bf16);
+    const gonn::WindowParts n = gonn::plan_window_bwd(p, D, is_bf16);
     uint8_t* w = (uint8_t*)round_up((size_t)ws, 256);
     p.lse2 = (float*)w;
     p.delta = (float*)(w + rows);
     p.part = (float*)(w + 2 * rows);
-    return 2 * rows + part + 256;
+    p.part_tail = p.part + n.part;
+    return 2 * rows + (n.part + n.tail) * sizeof(float) + 256;
 }
 
 // ---- helpers for the host shims ----------------------------------------

@@ -198,44 +198,64 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
 
 namespace {
 
-// The steps of a key block: query stages [st0, st0 + nst) of BQ rows for each of
-// the G query heads of its key head.
+// Keys of the tail's items, of which the sinks are the first (32; 64 where the stages
+// of four waves along the queries do not fit in LDS), and query rows per stage.
+constexpr int tail_keys(int D, bool f32) { return f32 && D == 128 ? 64 : 32; }
+constexpr int tail_rows(int D, bool f32) { return 4096 / tail_keys(D, f32); }
+
+// The steps of a key block: nst query stages of BQ rows, from q0 on, for each of the G
+// query heads of its key head.
 struct BlockSteps {
-    int st0, nst;
-    GONN_DEV void init(int k0, int BK, int BQ, int Sq, int kl, const Band& m) {
-        st0 = k0 / BQ;
-        int end = Sq;  // one past the last query that sees one of the keys
-        if (k0 >= m.sinks && Sq - k0 > BK - 1 + m.window) end = k0 + BK - 1 + m.window;
-        nst = k0 < kl && k0 < Sq ? (end + BQ - 1) / BQ - st0 : 0;
+    int q0, nst;
+    GONN_DEV void init(const WindowParams& p, int k0, int BK, int BQ, int kl, bool tail) {
+        if (tail) {  // the sinks' later queries
+            q0 = p.tail_q0;
+            nst = k0 < kl ? (p.Sq - q0 + BQ - 1) / BQ : 0;
+            return;
+        }
+        q0 = k0 / BQ * BQ;
+        int end = p.Sq;  // one past the last query that sees one of the keys
+        if ((k0 >= p.sinks || p.per_tail) && p.Sq - k0 > BK - 1 + p.window) end = k0 + BK - 1 + p.window;
+        nst = k0 < kl && k0 < p.Sq ? (end - q0 + BQ - 1) / BQ : 0;
     }
 };
 
-// One workgroup's share of the dK/dV grid: chunk c of key block kb of slice bk.
+// One workgroup's share of a dK/dV grid: chunk c of key block kb of slice bk.
 struct DkdvItem {
-    int bk, slot, kb, c, per, b, hk, G, kl;
-    GONN_DEV void init(const WindowParams& p) {
-        // Slots of a slice: the sinks' blocks first, per_sink items each.
-        map_block(blockIdx.x, p.slots, p.B * p.Hkv, false, bk, slot);
-        const int sink_slots = p.sink_blocks * p.per_sink;
-        const bool sink = slot < sink_slots;
-        per = sink ? p.per_sink : p.per_block;
-        const int i0 = sink ? slot : slot - sink_slots;
-        kb = (sink ? 0 : p.sink_blocks) + i0 / per;
-        c = i0 % per;
+    int bk, kb, c, b, hk, G, kl;
+    float* part;  // its partial, (2, BK, D), or null: it writes the gradients
+    GONN_DEV void init(const WindowParams& p, int BK, int D, bool tail) {
+        const int slots = tail ? p.per_tail : p.slots;
+        int slot;
+        map_block(blockIdx.x, slots, p.B * p.Hkv, false, bk, slot);
         b = bk / p.Hkv;
         hk = bk - b * p.Hkv;
         G = p.H / p.Hkv;
         kl = window_keys(p, b);
+        const size_t at = ((size_t)bk * slots + slot) * 2 * BK * D;
+        if (tail) {
+            kb = 0;
+            c = slot;
+            part = p.part_tail + at;
+            return;
+        }
+        // Slots of a slice: the sinks' blocks first, per_sink items each.
+        const int sink_slots = p.sink_blocks * p.per_sink;
+        const bool sink = slot < sink_slots;
+        const int per = sink ? p.per_sink : p.per_block, i0 = sink ? slot : slot - sink_slots;
+        kb = (sink ? 0 : p.sink_blocks) + i0 / per;
+        c = i0 % per;
+        part = per > 1 || (p.per_tail && kb == 0) ? p.part + at : nullptr;
     }
 };
 // dV and dK of key kj (row kj - k0 of the block), channels d .. d + 3: the gradients,
 // or one item's unscaled sums. live: the key takes part.
 template <int D, typename T>
-GONN_DEV void write_dkdv(const WindowParams& p, const DkdvItem& it, int BK, int kj, int k0, int d,
-                         f32x4 dv, f32x4 dk, bool live) {
+GONN_DEV void write_dkdv(const WindowParams& p, const DkdvItem& it, int BK, int kj, int d, f32x4 dv,
+                         f32x4 dk, bool live) {
     if (!live) dv = dk = f32x4{};
-    if (it.per > 1) {
-        float* part = p.part + (((size_t)it.bk * p.slots + it.slot) * 2 * BK + kj - k0) * D + d;
+    if (it.part) {
+        float* part = it.part + (size_t)(kj - it.kb * BK) * D + d;
         *(f32x4*)part = dv;
         *(f32x4*)(part + (size_t)BK * D) = dk;
     } else {
@@ -261,7 +281,7 @@ GONN_DEV void window_dkdv_plain(const WindowParams& p, const DkdvItem& it, const
             const size_t bh = (size_t)it.b * p.H + it.hk * it.G + st / bs.nst, base = bh * p.Sq;
 #pragma unroll 1
             for (int off = 0; off < BQ; off += 32) {
-                const int q0 = (bs.st0 + st % bs.nst) * BQ + off;
+                const int q0 = bs.q0 + st % bs.nst * BQ + off;
                 if (q0 >= p.Sq || !band.any(q0, q0 + 31, kw, kw + 31)) continue;
                 const size_t qr = (base + (q0 + ln < p.Sq ? q0 + ln : p.Sq - 1)) * D;
                 f32x16 s, dp;
@@ -291,14 +311,15 @@ GONN_DEV void window_dkdv_plain(const WindowParams& p, const DkdvItem& it, const
                     x[i] = dv[rq * 4 + i];
                     y[i] = dk[rq * 4 + i];
                 }
-                write_dkdv<D, T>(p, it, BK, kj, kw / BK * BK, 32 * t + 8 * rq + 4 * g, x, y, kj < it.kl);
+                write_dkdv<D, T>(p, it, BK, kj, 32 * t + 8 * rq + 4 * g, x, y, kj < it.kl);
             }
     }
 }
 
 }  // namespace
 
-template <int D, typename T, int WB, int NBUF, int OCC>
+// TAIL: the items of the sinks' later queries.
+template <int D, typename T, int WB, int NBUF, int OCC, bool TAIL = false>
 __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     constexpr int NS = 4 / WB, BK = WB * 32, BQ = NS * 32, NP = kPlanes<T>;
     constexpr int NKS = D / 16, NDT = D / 32;
@@ -311,23 +332,22 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = wave % WB, ws = wave / WB, g = lane >> 5, ln = lane & 31;
     DkdvItem it;
-    it.init(p);
-    const int bk = it.bk, b = it.b, hk = it.hk, G = it.G, kl = it.kl, per = it.per;
+    it.init(p, BK, D, TAIL);
+    const int bk = it.bk, b = it.b, hk = it.hk, G = it.G, kl = it.kl;
     const int k0 = it.kb * BK, kw = k0 + wb * 32, kj = kw + ln;
     const Band band{p.window, p.sinks};
     BlockSteps bs;
-    bs.init(k0, BK, BQ, p.Sq, kl, band);
-    const int s0 = it.c * p.chunk;
-    int s1 = bs.nst * G;
-    s1 = per > 1 && s1 - s0 > p.chunk ? s0 + p.chunk : s1;
-    if (per > 1 && s0 >= s1) return;  // no such item: nothing is read from its slot
+    bs.init(p, k0, BK, BQ, kl, TAIL);
+    const int chunk = TAIL ? p.tail_chunk : p.chunk, s0 = it.c * chunk;
+    const int s1 = bs.nst * G - s0 > chunk ? s0 + chunk : bs.nst * G;
+    if (it.part && s0 >= s1) return;  // no such item: nothing is read from its slot
 
     Stage in;
     in.init(tid);
     float rl = 0.f, rd = 0.f;
     auto gload = [&](int st) {
         const size_t bh = (size_t)b * p.H + hk * G + st / bs.nst;
-        const int q0 = (bs.st0 + st % bs.nst) * BQ;
+        const int q0 = bs.q0 + st % bs.nst * BQ;
         in.load((const T*)p.q + bh * p.Sq * D, (const T*)p.dO + bh * p.Sq * D, q0, p.Sq);
         if (tid < BQ) {
             const int q = q0 + tid;
@@ -355,7 +375,7 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     const float c2 = p.scale_log2;
 
     auto compute = [&](int st, int buf) {
-        const int q0 = (bs.st0 + st % bs.nst) * BQ + ws * 32;
+        const int q0 = bs.q0 + st % bs.nst * BQ + ws * 32;
         if (q0 >= p.Sq || !band.any(q0, q0 + 31, kw, kw + 31)) return;  // wave-uniform
         char* tile = smem + buf * STAGE + ws * Stage::TILE;
         f32x16 s = f32x16{}, dp = f32x16{};
@@ -425,7 +445,7 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
                 x[i] = acc[t][rq * 4 + i];
                 y[i] = acc[NDT + t][rq * 4 + i];
             }
-            write_dkdv<D, T>(p, it, BK, kj, k0, t * 32 + rq * 8 + g * 4, x, y, kj < kl);
+            write_dkdv<D, T>(p, it, BK, kj, t * 32 + rq * 8 + g * 4, x, y, kj < kl);
         }
 }
 
@@ -465,20 +485,20 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_pipe_kernel(WindowParams p
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 5, ln = lane & 31;
     DkdvItem it;
-    it.init(p);
+    it.init(p, BK, D, false);
     const int k0 = it.kb * BK, kw = k0 + wave * 32, kj = kw + ln, kl = it.kl;
     const Band band{p.window, p.sinks};
     BlockSteps bs;
-    bs.init(k0, BK, BQ, p.Sq, kl, band);
+    bs.init(p, k0, BK, BQ, kl, false);
     const int s0 = it.c * p.chunk;
     int nq = bs.nst * it.G - s0;
-    nq = it.per > 1 && nq > p.chunk ? p.chunk : nq;
+    nq = nq > p.chunk ? p.chunk : nq;
     if (nq <= 0) {  // no such item, or no query sees the block
-        if (it.per > 1) return;
+        if (it.part) return;
         for (int i = tid; i < BK * D / 4; i += 256) {
             const int r = i / (D / 4);
             if (k0 + r < p.Sk)
-                write_dkdv<D, bf16>(p, it, BK, k0 + r, k0, i % (D / 4) * 4, f32x4{}, f32x4{}, false);
+                write_dkdv<D, bf16>(p, it, BK, k0 + r, i % (D / 4) * 4, f32x4{}, f32x4{}, false);
         }
         return;
     }
@@ -510,7 +530,7 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_pipe_kernel(WindowParams p
     struct Cursor {
         int hh, qt;
     };
-    const int st0 = bs.st0, stE = bs.st0 + bs.nst;
+    const int st0 = bs.q0 / BQ, stE = st0 + bs.nst;
     auto next = [&](Cursor c) {
         c.qt++;
         if (c.qt == stE) {
@@ -781,7 +801,7 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_pipe_kernel(WindowParams p
                 x[k] = dvacc[t][rq4 * 4 + k];
                 y[k] = dkacc[t][rq4 * 4 + k];
             }
-            write_dkdv<D, bf16>(p, it, BK, kj, k0, t * 32 + rq4 * 8 + g * 4, x, y, kj < kl);
+            write_dkdv<D, bf16>(p, it, BK, kj, t * 32 + rq4 * 8 + g * 4, x, y, kj < kl);
         }
 }
 
@@ -800,18 +820,26 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowParams p, int BK
     r /= BK;
     const int kb = (int)(r % nb), bk = (int)(r / nb), b = bk / p.Hkv, kj = kb * BK + row;
     if (kj >= p.Sk) return;
-    const bool sink = kb < p.sink_blocks;
+    const bool sink = kb < p.sink_blocks, tail = p.per_tail && kb == 0;
     const int per = sink ? p.per_sink : p.per_block;
-    if (per == 1) return;  // written by its item
+    if (per == 1 && !tail) return;  // written by its item
     const int slot = sink ? kb * per : p.sink_blocks * p.per_sink + (kb - p.sink_blocks) * per;
     int kl = p.kv_len ? p.kv_len[b] : p.Sk;
     kl = kl < 0 ? 0 : (kl > p.Sk ? p.Sk : kl);
+    const int G = p.H / p.Hkv;
     BlockSteps bs;
-    bs.init(kb * BK, BK, BQ, p.Sq, kl, {p.window, p.sinks});
-    const int cnt = (bs.nst * (p.H / p.Hkv) + p.chunk - 1) / p.chunk;
+    bs.init(p, kb * BK, BK, BQ, kl, false);
+    const int cnt = (bs.nst * G + p.chunk - 1) / p.chunk;
     const float* src = p.part + (((size_t)bk * p.slots + slot) * 2 * BK + w * BK + row) * D + d;
     f32x4 sum = f32x4{};
     for (int c = 0; c < cnt; c++) sum += *(const f32x4*)(src + (size_t)c * 2 * BK * D);
+    constexpr int TK = tail_keys(D, sizeof(T) == 4);
+    if (tail && row < TK) {
+        bs.init(p, 0, TK, tail_rows(D, sizeof(T) == 4), kl, true);
+        const int n = (bs.nst * G + p.tail_chunk - 1) / p.tail_chunk;
+        src = p.part_tail + (((size_t)bk * p.per_tail) * 2 * TK + w * TK + row) * D + d;
+        for (int c = 0; c < n; c++) sum += *(const f32x4*)(src + (size_t)c * 2 * TK * D);
+    }
     if (w) sum *= p.scale;
     store4<T>((T*)(w ? p.dk : p.dv) + ((size_t)bk * p.Sk + kj) * D + d, sum);
 }
@@ -840,8 +868,11 @@ void run_dkdv(const WindowParams& p, int BK, int BQ, hipStream_t s) {
     } else {
         window_dkdv_kernel<D, T, 2, 1, 1><<<grid, 256, 0, s>>>(p);
     }
+    if (p.per_tail)
+        window_dkdv_kernel<D, T, tail_keys(D, sizeof(T) == 4) / 32, sizeof(T) == 2 ? 2 : 1, 1, true>
+            <<<(unsigned)p.per_tail * (unsigned)(p.B * p.Hkv), 256, 0, s>>>(p);
     const int nkb = (p.Sk + BK - 1) / BK;
-    const int nb = p.per_block > 1 ? nkb : (p.per_sink > 1 ? p.sink_blocks : 0);
+    const int nb = p.per_block > 1 ? nkb : p.per_tail ? 1 : p.per_sink > 1 ? p.sink_blocks : 0;
     if (!nb) return;
     const size_t n = (size_t)p.B * p.Hkv * nb * BK * 2 * (D / 4);
     window_join_kernel<D, T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p, BK, BQ, nb, n);
@@ -864,14 +895,27 @@ void run_window_bwd(const WindowParams& p, hipStream_t s) {
 
 }  // namespace
 
-size_t plan_window_bwd(WindowParams& p, int D, int is_bf16) {
+WindowParts plan_window_bwd(WindowParams& p, int D, int is_bf16) {
     const DkdvShape sh = dkdv_shape(p, D, is_bf16);
     const long long slices = (long long)p.B * p.Hkv, G = p.H / p.Hkv, want = 2 * device_cus();
     const int nkb = (p.Sk + sh.BK - 1) / sh.BK;
     const long long all = G * ((p.Sq + sh.BQ - 1) / sh.BQ);
-    const long long band = std::min<long long>(
-        all, G * (((long long)sh.BK - 1 + p.window + sh.BQ - 1) / sh.BQ + 1));
+    const long long stages = ((long long)sh.BK - 1 + p.window + sh.BQ - 1) / sh.BQ;
+    const long long band = std::min<long long>(all, G * (stages + 1));
+    // Sinks are read by every later query. Up to 32 of them (one tile) have those
+    // queries in items of 32 keys and four waves along the queries; with more, their
+    // blocks have all queries and more items.
+    const long long tail_q0 = stages * sh.BQ;
+    p.per_tail = 0;
     p.sink_blocks = std::min(nkb, (p.sinks + sh.BK - 1) / sh.BK);
+    if (p.sinks > 0 && p.sinks <= 32 && tail_q0 < p.Sq) {
+        p.sink_blocks = 0;
+        p.tail_q0 = (int)tail_q0;
+        const int rows = tail_rows(D, !is_bf16);
+        const long long steps = G * ((p.Sq - tail_q0 + rows - 1) / rows);
+        p.tail_chunk = (int)std::max<long long>(2, (steps * slices + want / 2 - 1) / (want / 2));
+        p.per_tail = (int)((steps + p.tail_chunk - 1) / p.tail_chunk);
+    }
     // Items as long as a block's band, shorter where that leaves the device
     // without work, but no shorter than 4 stages.
     const long long items = slices * nkb;
@@ -882,10 +926,10 @@ size_t plan_window_bwd(WindowParams& p, int D, int is_bf16) {
     p.per_block = (int)((band + chunk - 1) / chunk);
     p.per_sink = (int)((all + chunk - 1) / chunk);
     p.slots = p.sink_blocks * p.per_sink + (nkb - p.sink_blocks) * p.per_block;
-    const size_t part = p.per_block > 1 || (p.sink_blocks && p.per_sink > 1)
-                            ? (size_t)slices * p.slots * 2 * sh.BK * D * sizeof(float)
-                            : 0;
-    return part;
+    WindowParts n{0, (size_t)slices * p.per_tail * 2 * tail_keys(D, !is_bf16) * D};
+    if (p.per_block > 1 || (p.sink_blocks && p.per_sink > 1) || p.per_tail)
+        n.part = (size_t)slices * p.slots * 2 * sh.BK * D;
+    return n;
 }
 
 hipError_t launch_window_bwd(const WindowParams& p, int D, int is_bf16, hipStream_t s) {

@@ -158,10 +158,19 @@ struct WindowParams {
     // partials, (B*Hkv, slots, 2, keys, D) f32, that a second kernel adds up.
     float* part;
     int chunk, per_block, per_sink, sink_blocks, slots;
+    // Up to 32 sinks: the queries from tail_q0 on, which see nothing else of the first
+    // key block, in items of their own, per_tail of tail_chunk steps for each slice,
+    // with partials like `part`'s. per_tail 0: none.
+    float* part_tail;
+    int tail_q0, tail_chunk, per_tail;
 };
 hipError_t launch_window_fwd(const WindowParams& p, int D, int is_bf16, hipStream_t s);
-// Fills the work items of the dK/dV kernel; returns the bytes of p.part.
-size_t plan_window_bwd(WindowParams& p, int D, int is_bf16);
+// Fills the work items of the dK/dV kernels; returns the floats of p.part and, behind
+// them, of p.part_tail.
+struct WindowParts {
+    size_t part, tail;
+};
+WindowParts plan_window_bwd(WindowParams& p, int D, int is_bf16);
 hipError_t launch_window_bwd(const WindowParams& p, int D, int is_bf16, hipStream_t s);
 
 // Exact fp64 attention (attn_f64.hip): fp64 (BH, rows, d) buffers.

@@ -29,6 +29,8 @@ CASES = [
     (8, 64, 32, 300, 300, 64, 40, 5, (300, 1, 64, 128, 129, 200, 299, 0)),
     (4, 64, 32, 260, 300, 128, 100, 140, None),
     (2, 32, 16, 1100, 1100, 64, 128, 4, None),
+    (2, 32, 16, 1100, 1100, 128, 70, 32, (1100, 20)),
+    (1, 3, 1, 700, 640, 128, 50, 7, None),           # queries past every key but the sinks
 ]
 
 
@@ -96,9 +98,10 @@ def test_gradients_against_differences():
 
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
-def test_scales(scale, dtype):
+@pytest.mark.parametrize("big", [False, True])
+def test_scales(scale, dtype, big):
     from gonn_amd import hip
-    c = (1, 2, 1, 100, 100, 64, 30, 4, None)
+    c = (16, 32, 16, 100, 100, 64, 30, 4, None) if big else (1, 2, 1, 100, 100, 64, 30, 4, None)
     q, k, v, dO = _data(c, dtype, 7)
     if scale == 3.0:
         q *= 0.25
