@@ -229,6 +229,312 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
                                   oacc[t][rq * 4 + 3]}, m, lt);
 }
 
+// ---------------------------------------------------------------------------
+// bf16 forward of large grids: the three-stage pipeline of attn_fwd.hip (4 waves, 128
+// query rows, 64-key tiles) on the two runs of tiles. Step t issues
+//   MFMA  O^T += V(t)^T P(t)
+//   MFMA  S^T(t+2) = K(t+2) Q^T
+//   VALU  P(t+1) = exp2(S^T(t+1) c2 - mc), packed to bf16, and its row sums
+// K and V tiles go straight from memory to two-slot LDS rings, row-major (V^T is read
+// with ds_read_b64_tr_b16, so nothing is packed beforehand). Scores stay unscaled and
+// exact; P is exact for any offset mc, which only has to keep it bounded: a tile whose
+// row sum exceeds 2^14, or a row that has seen nothing yet, takes a rare branch that
+// moves mc to the tile's maximum. Rows sum the unrounded P, so that LSE keeps fp32
+// accuracy. The scale's sign goes into Q.
+// ---------------------------------------------------------------------------
+constexpr float kSumBound = 16384.f, kLazyLog2 = 8.f;
+
+template <int D>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_fwd_pipe_kernel(WindowParams p) {
+    constexpr int NW = 4, BM = NW * 32, BN = 64, NT = NW * 64;
+    constexpr int NKS = D / 16, NDT = D / 32;
+    constexpr uint32_t TB = BN * D * 2;  // bytes of a K or V tile
+    constexpr int KLEAD = 3, VLEAD = 1;
+    __shared__ __attribute__((aligned(16))) bf16 sKb[2 * BN * D];
+    __shared__ __attribute__((aligned(16))) bf16 sVb[2 * BN * D];
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 5, ln = lane & 31;
+    int bh, qb;
+    map_block(blockIdx.x, (p.Sq + BM - 1) / BM, p.B * p.H, true, bh, qb);
+    const int b = bh / p.H, h = bh - b * p.H, bk = b * p.Hkv + h / (p.H / p.Hkv);
+    const int Sq = p.Sq, q0 = qb * BM, qw = q0 + wave * 32, qi = qw + ln, kl = window_keys(p, b);
+    const Band band{p.window, p.sinks};
+    KeyStages ks_;
+    ks_.init(q0, q0 + BM < Sq ? q0 + BM : Sq, kl, BN, band);
+    const int ntiles = ks_.count();
+    if (ntiles == 0) {  // uniform: no row sees a key
+        for (int i = tid; i < BM * D / 4; i += NT) {
+            const int r = i / (D / 4);
+            if (q0 + r < Sq)
+                write_row<D, bf16>(p, (size_t)bh * Sq + q0 + r, i % (D / 4) * 4, f32x4{}, 0.f, 0.f);
+        }
+        return;
+    }
+    const float c2 = p.c2;
+
+    bf16x8 qf[NKS];
+    auto load_q = [&]() {
+        const bf16* qrow = (const bf16*)p.q + ((size_t)bh * Sq + (qi < Sq ? qi : Sq - 1)) * D + g * 8;
+        const uint32_t flip = p.sign < 0.f ? 0x80008000u : 0u, keep = p.sign != 0.f ? ~0u : 0u;
+        for (int ks = 0; ks < NKS; ks++) {
+            u32x4 a = *(const u32x4*)(qrow + ks * 16);
+            for (int e = 0; e < 4; e++) a[e] = (a[e] ^ flip) & keep;
+            qf[ks] = __builtin_bit_cast(bf16x8, a);
+        }
+    };
+
+    // Tile loads: instruction i of thread tid fills 16-byte position i * NT + tid.
+    constexpr int NI = BN * D / 8 / NT;  // loads of a tile
+    uint32_t toff[NI];
+    for (int i = 0; i < NI; i++) {
+        int r, c;
+        slab_chunk(i * NT + tid, BN, r, c);
+        toff[i] = (uint32_t)((r * D + c * 8) * 2);
+    }
+    // Keys at and past kl read as zeros.
+    const brsrc krs = make_rsrc((const bf16*)p.k + (size_t)bk * p.Sk * D, (uint32_t)kl * D * 2);
+    const brsrc vrs = make_rsrc((const bf16*)p.v + (size_t)bk * p.Sk * D, (uint32_t)kl * D * 2);
+    const uint32_t kl0 = lds_addr(sKb) + wave * 1024, vl0 = lds_addr(sVb) + wave * 1024;
+    auto clamped = [&](int t) { return (uint32_t)ks_.stage(t < ntiles ? t : ntiles - 1) * TB; };
+    auto dma = [&](brsrc rs, uint32_t base, uint32_t so) {
+        for (int i = 0; i < NI; i++) dma16(rs, base + i * NT * 16, toff[i], so);
+    };
+
+    const int hs = slab_swz(ln);
+    const uint32_t qa0 = (uint32_t)(ln * 64 + ((0 + g) ^ hs) * 16);
+    const uint32_t qa1 = (uint32_t)(ln * 64 + ((2 + g) ^ hs) * 16);
+    const int s16 = lane & 15, tcx = 2 * ((ln >> 4) & 1) + ((s16 >> 1) & 1);
+    const uint32_t ta0 = (uint32_t)((4 * g + (s16 >> 2)) * 64 + (tcx ^ g) * 16 + 8 * (s16 & 1));
+    const uint32_t ta1 =
+        (uint32_t)((8 + 4 * g + (s16 >> 2)) * 64 + (tcx ^ (2 + g)) * 16 + 8 * (s16 & 1));
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    typedef __attribute__((address_space(3))) char lds_char;
+    const char* sKc = (const char*)sKb;
+    lds_char* const sVc = (lds_char*)sVb;
+    auto kfrag = [&](const char* tile, int ks, int mt) {
+        return *(const bf16x8*)(tile + ((ks & 1) ? qa1 : qa0) + ((ks >> 1) * BN + mt * 32) * 64);
+    };
+    auto vfrag = [&](uint32_t base, int ks, int dt) {
+        lds_char* const x = sVc + base + (dt * BN + 16 * ks) * 64;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(x + ta0));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(x + ta1));
+        const s4 b8[2] = {lo, hi};
+        return __builtin_bit_cast(bf16x8, b8);
+    };
+
+    f32x16 oacc[NDT];
+    for (int dt = 0; dt < NDT; dt++) oacc[dt] = f32x16{};
+    float mc = 0.f, l = 0.f, alpha = 1.f;
+
+    // Scores of tile t that this lane's row does not see, to -inf (c2 > 0).
+    auto mask = [&](int t, f32x16* s) {
+        const int kb = ks_.stage(t) * BN;
+        if (kb + BN <= kl && band.all(qw, qw + 31, kb, kb + BN - 1)) return;  // wave-uniform
+        // Key 32 mt + 8 (r / 4) + r % 4 of the lane group: up to hi, and past lo or below sk.
+        const int base = kb + 4 * g, hi = (qi < kl - 1 ? qi : kl - 1) - base;
+        const int lo = qi - p.window - base, sk = p.sinks - base;
+        for (int mt = 0; mt < 2; mt++)
+            for (int r = 0; r < 16; r++) {
+                const int c = mt * 32 + 8 * (r >> 2) + (r & 3);
+                s[mt][r] = c > hi || (c <= lo && c >= sk) ? -INFINITY : s[mt][r];
+            }
+    };
+    // Maximum of a tile's scaled scores over the row.
+    auto tile_max = [&](const f32x16* s) {
+        float m0 = -INFINITY;
+        for (int mt = 0; mt < 2; mt++)
+            for (int r = 0; r < 16; r++) m0 = fmaxf(m0, s[mt][r]);
+        return pair_max32(m0) * c2;
+    };
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    auto p_tile = [&](const f32x16* s, u32x4* pk) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 16; k++) {
+            const int mt = k >> 3, r = (k & 7) * 2;
+            const float a = fast_exp2(__builtin_fmaf(s[mt][r], c2, -mc));
+            const float c = fast_exp2(__builtin_fmaf(s[mt][r + 1], c2, -mc));
+            part[k & 3] += a + c;
+            const bf16x2 pr = {to_bf16(a), to_bf16(c)};
+            pk[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, pr);
+        }
+        return (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    u32x4 pp[4];  // P of the tile PV consumes next
+
+    // One step, scheduled by hand as in attn_fwd.hip. TAIL: 0 a full step; 1 the
+    // next-to-last (no S^T(t+2)); 2 the last (no P(t+1) either).
+    auto step = [&](int t, f32x16* sA, f32x16* sB, auto TAILC) __attribute__((always_inline)) {
+        constexpr int TAIL = decltype(TAILC)::value;
+        const uint32_t kso = clamped(t + KLEAD), vso = clamped(t + VLEAD);
+        const int kslot = (t + KLEAD) & 1, vslot = (t + 1) & 1;
+        if constexpr (TAIL < 2) mask(t + 1, sB);
+        const uint32_t vb = (uint32_t)(t & 1) * TB;
+        const char* kt = sKc + (uint32_t)(t & 1) * TB;
+
+        constexpr int SKS = NKS / 4, GW = NDT + 2 * SKS, NM = 4 * GW, NU = 16, LA = 3;
+        constexpr int NDMA = 2 * NI, DS = 2;
+        static_assert(DS * NDMA <= NM, "the step's tile loads fit in its slots");
+        bf16x8 opr[4];
+        auto fetch = [&](auto E) {
+            constexpr int e = decltype(E)::value, j = e / GW, w = e % GW;
+            if constexpr (w < NDT) opr[e & 3] = vfrag(vb, j, w);
+            else if constexpr (TAIL == 0)
+                opr[e & 3] = kfrag(kt, SKS * j + ((w - NDT) >> 1), (w - NDT) & 1);
+        };
+        auto issue = [&](auto E) {
+            constexpr int e = decltype(E)::value, j = e / GW, w = e % GW;
+            if constexpr (w < NDT) {
+                oacc[w] = mfma_bf16(opr[e & 3], __builtin_bit_cast(bf16x8, pp[j]), oacc[w]);
+            } else if constexpr (TAIL == 0) {
+                constexpr int kk = SKS * j + ((w - NDT) >> 1), mt = (w - NDT) & 1;
+                sA[mt] = mfma_bf16(opr[e & 3], qf[kk], kk == 0 ? f32x16{} : sA[mt]);
+            }
+        };
+        auto dma_slot = [&](auto E) {
+            constexpr int e = decltype(E)::value;
+            constexpr int d0 = TAIL == 0 ? 0 : (TAIL == 1 ? NI : NDMA);
+            if constexpr (e % DS == 0 && e / DS < NDMA && e / DS >= d0) {
+                constexpr int d = e / DS;
+                dma_set_m0(d < NI ? kl0 + kslot * TB + d * NT * 16 : vl0 + vslot * TB + (d - NI) * NT * 16);
+            }
+            if constexpr (e >= 1 && (e - 1) % DS == 0 && (e - 1) / DS < NDMA && (e - 1) / DS >= d0) {
+                constexpr int d = (e - 1) / DS;
+                if constexpr (d < NI) dma16_m0(krs, toff[d], kso);
+                else dma16_m0(vrs, toff[d - NI], vso);
+            }
+        };
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        auto uslot = [](int k) { return (k >> 2) * GW + NDT + (k & 3); };
+        float ub[16][2];
+        auto uop = [&](auto U, auto S) {
+            constexpr int k = decltype(U)::value, stage = decltype(S)::value;
+            constexpr int mt = k >> 3, r = (k & 7) * 2;
+            if constexpr (stage == 0) {
+                ub[k][0] = fast_exp2(__builtin_fmaf(sB[mt][r], c2, -mc));
+                ub[k][1] = fast_exp2(__builtin_fmaf(sB[mt][r + 1], c2, -mc));
+                pin(ub[k][0]);
+                pin(ub[k][1]);
+            } else {
+                part[k & 3] += ub[k][0] + ub[k][1];
+                const bf16x2 pr = {to_bf16(ub[k][0]), to_bf16(ub[k][1])};
+                pp[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, pr);
+                pin(pp[k >> 2][k & 3]);
+                pin(part[k & 3]);
+            }
+        };
+        auto uops_at = [&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (TAIL == 2) return;
+            static_for<2>([&](auto S) {
+                static_for<NU>([&](auto U) {
+                    constexpr int at = uslot(decltype(U)::value) - 2 + 2 * decltype(S)::value;
+                    if constexpr (e < NM ? at == e : at >= NM) uop(U, S);
+                });
+            });
+        };
+        __builtin_amdgcn_s_setprio(1);
+        static_for<LA>([&](auto E) { fetch(E); });
+        static_for<NM>([&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (e + LA < NM) fetch(std::integral_constant<int, e + LA>{});
+            issue(E);
+            dma_slot(E);
+            uops_at(E);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        uops_at(std::integral_constant<int, NM>{});
+        __builtin_amdgcn_s_setprio(0);
+        float ts = (part[0] + part[1]) + (part[2] + part[3]);
+        alpha = 1.f;
+        if (TAIL < 2 && __builtin_amdgcn_ballot_w64(!(ts <= kSumBound) || l == 0.f)) {
+            const float mx = tile_max(sB);
+            const bool empty = pair_sum32(l) == 0.f;
+            const float mn = mx > -INFINITY && (empty || mx - mc > kLazyLog2) ? mx : mc;
+            alpha = empty ? 0.f : fast_exp2(mc - mn);
+            mc = mn;
+            ts = p_tile(sB, pp);
+        }
+        l = l * alpha + ts;
+        if constexpr (TAIL == 0) {  // S^T(t+2) is read behind the branches below
+            pin_before_branch(sA[0]);
+            pin_before_branch(sA[1]);
+        }
+        GONN_VMCNT(0);
+        __syncthreads();
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.f))
+            for (int dt = 0; dt < NDT; dt++) oacc[dt] *= alpha;
+    };
+
+    // Prologue: S^T(0) -> P(0), S^T(1); K(0) is staged in V slot 1.
+    f32x16 s0[2], s1[2];
+    auto qk_tile = [&](const char* tile, f32x16* s) {
+        s[0] = s[1] = f32x16{};
+        for (int ks = 0; ks < NKS; ks++)
+            for (int mt = 0; mt < 2; mt++) s[mt] = mfma_bf16(kfrag(tile, ks, mt), qf[ks], s[mt]);
+    };
+    dma(krs, vl0 + TB, clamped(0));
+    dma(krs, kl0 + TB, clamped(1));
+    dma(krs, kl0, clamped(2));
+    dma(vrs, vl0, clamped(0));
+    load_q();
+    GONN_VMCNT(0);
+    __syncthreads();
+    qk_tile((const char*)sVb + TB, s0);
+    qk_tile(sKc + TB, s1);
+    for (int mt = 0; mt < 2; mt++) {
+        pin_before_branch(s0[mt]);
+        pin_before_branch(s1[mt]);
+    }
+    mask(0, s0);
+    mc = tile_max(s0);
+    if (!(mc > -INFINITY)) mc = 0.f;  // nothing seen yet: no offset
+    l = p_tile(s0, pp);
+    __syncthreads();  // K(0) and K(1) read by every wave
+
+    {
+        const std::integral_constant<int, 0> full;
+        const std::integral_constant<int, 1> tail1;
+        const std::integral_constant<int, 2> tail2;
+        const int nfull = ntiles - 2;
+        int t = 0;
+        for (; t + 1 < nfull; t += 2) {
+            step(t, s0, s1, full);
+            step(t + 1, s1, s0, full);
+        }
+        if (t < nfull) step(t++, s0, s1, full);
+        if (ntiles >= 2) {
+            if (t & 1)
+                for (int mt = 0; mt < 2; mt++) {
+                    const f32x16 x = s0[mt];
+                    s0[mt] = s1[mt];
+                    s1[mt] = x;
+                }
+            step(t, s0, s1, tail1);
+        }
+        step(ntiles - 1, s1, s0, tail2);
+    }
+    GONN_VMCNT(0);  // loads in flight write this workgroup's LDS
+
+    const float lt = pair_sum32(l);
+    bool bad = nonfinite(lt);
+    for (int t = 0; t < NDT; t++)
+        for (int r = 0; r < 16; r++) bad |= nonfinite(oacc[t][r]);
+    if (__builtin_amdgcn_ballot_w64(bad && qi < Sq)) {
+        window_fwd_plain<D, bf16>(p, bh, bk, kl, band, qw);
+        return;
+    }
+    if (qi >= Sq) return;
+    const size_t row = (size_t)bh * Sq + qi;
+    for (int t = 0; t < NDT; t++)
+        for (int rq = 0; rq < 4; rq++)
+            write_row<D, bf16>(p, row, t * 32 + rq * 8 + g * 4,
+                               f32x4{oacc[t][rq * 4], oacc[t][rq * 4 + 1], oacc[t][rq * 4 + 2],
+                                     oacc[t][rq * 4 + 3]}, mc, lt);
+}
+
 namespace {
 
 template <int D, typename T, int WQ, int NBUF, int OCC>
@@ -243,7 +549,9 @@ void pick_window_fwd(const WindowParams& p, hipStream_t s) {
     const long long b128 = (long long)((p.Sq + 127) / 128) * BH;
     const long long b64 = (long long)((p.Sq + 63) / 64) * BH;
     if constexpr (sizeof(T) == 2) {
-        if (b128 >= 2 * cus) run_window_fwd<D, T, 4, 2, 2>(p, s);
+        // The pipelined kernel reads a head's keys with 32-bit offsets.
+        const bool near = (double)p.Sk * D * 2 < 4.0e9;
+        if (b128 >= 2 * cus && near) window_fwd_pipe_kernel<D><<<(unsigned)b128, 256, 0, s>>>(p);
         else if (b64 >= cus) run_window_fwd<D, T, 2, 2, 2>(p, s);
         else run_window_fwd<D, T, 1, 2, 1>(p, s);
     } else {
