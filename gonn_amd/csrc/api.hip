@@ -2030,8 +2030,9 @@ int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D)
     const size_t BH = (size_t)B * H, codes = BH * c.nblk * gonn::kBlk8 * D,
                  ring = BH * 2 * gonn::kBlk8 * D * sizeof(uint16_t),
                  scales = round_up(BH * c.nblk * sizeof(float), 256),
-                 lens = round_up((size_t)B * sizeof(int), 256);
-    const size_t bytes = 2 * codes + 2 * scales + 2 * ring + 3 * lens;
+                 lens = round_up((size_t)B * sizeof(int), 256),
+                 tickets = (size_t)B * gonn::kTicketStep8 * sizeof(unsigned);
+    const size_t bytes = 2 * codes + 2 * scales + 2 * ring + 2 * lens + tickets;
     if (hipMalloc(&h->mem, bytes) != hipSuccess) {
         (void)hipGetLastError();
         delete h;
@@ -2052,8 +2053,8 @@ int gonn_hip_kvcache8_create(gonn_kvcache8** out, int B, int H, int Lmax, int D)
     uint8_t* state = p;
     c.len = (int*)take(lens);
     c.lo = (int*)take(lens);
-    c.ticket = (unsigned*)take(lens);
-    hipError_t e = hipMemset(state, 0, 3 * lens);
+    c.ticket = (unsigned*)take(tickets);
+    hipError_t e = hipMemset(state, 0, 2 * lens + tickets);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         (void)hipFree(h->mem);

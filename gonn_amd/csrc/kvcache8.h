@@ -17,6 +17,7 @@ namespace gonn {
 
 constexpr int kBlk8 = 64;           // positions per block
 constexpr int kLeastExp8 = -100;    // least exponent of a scale
+constexpr int kTicketStep8 = 32;    // counters of different sequences: 128 bytes apart
 constexpr int kSeqs8 = 256;         // sequences per append or truncate launch
 
 struct Cache8 {
@@ -28,7 +29,7 @@ struct Cache8 {
     uint16_t* vt;  // (B*H, 2, D, 64) bf16: position p at (p / 64 % 2, :, p % 64)
     int* len;      // [B]
     int* lo;       // [B] first position whose bf16 row the ring still holds
-    unsigned* ticket;  // [B] workgroups of a running append that have read len
+    unsigned* ticket;  // (B, kTicketStep8) workgroups of a running append that have read len
     int B, H, Lmax, D, nblk;
 };
 

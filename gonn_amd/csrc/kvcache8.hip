@@ -92,8 +92,16 @@ __global__ __launch_bounds__(256) void append8_kernel(Cache8 c, const T* __restr
                 if (keep) *(u16x8*)(kring + (size_t)r * D + d) = kx[j];
             } else if (closing) {  // an older row, from the ring
                 kx[j] = *(const u16x8*)(kring + (size_t)r * D + d);
+            }
+        }
+        if (closing && p0 > base) {  // older values, eight positions of a channel at a time
+            const int old = p0 - base;
+            for (int ch = tid; ch < D * 8; ch += 256) {
+                const int d = ch >> 3, r = (ch & 7) * 8;
+                if (r >= old) continue;
+                const u16x8 v = *(const u16x8*)(vring + ch * 8);
                 for (int e = 0; e < 8; e++)
-                    vtile[(d + e) * VS + r] = vring[(size_t)(d + e) * kBlk8 + r];
+                    if (r + e < old) vtile[d * VS + r + e] = v[e];
             }
         }
         __syncthreads();
@@ -159,14 +167,16 @@ __global__ __launch_bounds__(256) void append8_kernel(Cache8 c, const T* __restr
     }
     if constexpr (RING) {
         // The length was read above (the branches waited for it); the last of the
-        // sequence's workgroups to say so advances it. One counter per sequence:
-        // updates of one address take about 40 ns each, 2048 on one 84 us.
+        // sequence's workgroups to say so advances it. One counter, and one cache
+        // line, per sequence: updates of one address take about 40 ns each, 2048 on
+        // one 84 us.
         __syncthreads();
-        if (tid == 0 && atomicAdd(c.ticket + b, 1u) == (unsigned)(c.H * nb) - 1) {
+        unsigned* ticket = c.ticket + (size_t)b * kTicketStep8;
+        if (tid == 0 && atomicAdd(ticket, 1u) == (unsigned)(c.H * nb) - 1) {
             const int first = (end / kBlk8 - 1) * kBlk8;
             c.len[b] = end;
             if (first > c.lo[b]) c.lo[b] = first;
-            c.ticket[b] = 0;
+            *ticket = 0;
         }
     }
 }
