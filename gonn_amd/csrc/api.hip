@@ -862,7 +862,7 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     // TB/s, 32 6.2, 64 6.6, 128 6.9), but sequences of different lengths level out
     // less (512 to 8192: 441, 397, 387, 390 us). Shorter ones where the device has
     // room for more workgroups, down to a block per key wave.
-    const long long want = 4 * cus, least = p.rows <= 32 ? 4 : 128 / p.rows;
+    const long long want = (p.rows == 128 ? 2 : 4) * cus, least = p.rows <= 32 ? 4 : 128 / p.rows;
     long long split = 64;
     if (units * ((blocks + split - 1) / split) < want)
         split = std::min(split, std::max(least, blocks * units / want));
@@ -2177,6 +2177,9 @@ int gonn_hip_kvcache8_attend(gonn_kvcache8* h, const gonn_buf* q, gonn_buf* o, i
     a.split = plan.split;
     a.nsplit = plan.nsplit;
     a.scale_log2 = (float)(scale * 1.4426950408889634);
+    const QFold qf = q_fold(scale);
+    a.c2 = qf.c2;
+    a.sign = qf.sign;
     float* w = (float*)round_up((size_t)ws, 256);
     a.part_ml = w;
     a.part_o = w + round_up((size_t)h->c.B * Hq * T * plan.nsplit * 2, 64);

@@ -458,10 +458,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_fwd_pipe_kernel(W
             ts = p_tile(sB, pp);
         }
         l = l * alpha + ts;
-        if constexpr (TAIL == 0) {  // S^T(t+2) is read behind the branches below
-            pin_before_branch(sA[0]);
-            pin_before_branch(sA[1]);
-        }
         GONN_VMCNT(0);
         __syncthreads();
         if (__builtin_amdgcn_ballot_w64(alpha != 1.f))
@@ -484,10 +480,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void window_fwd_pipe_kernel(W
     __syncthreads();
     qk_tile((const char*)sVb + TB, s0);
     qk_tile(sKc + TB, s1);
-    for (int mt = 0; mt < 2; mt++) {
-        pin_before_branch(s0[mt]);
-        pin_before_branch(s1[mt]);
-    }
+    settle_before_branch(s0[0], s0[1]);
+    settle_before_branch(s1[0], s1[1]);
     mask(0, s0);
     mc = tile_max(s0);
     if (!(mc > -INFINITY)) mc = 0.f;  // nothing seen yet: no offset

@@ -327,6 +327,10 @@ template <typename T>
 GONN_DEV void pin_before_branch(const T& x) {
     pin(x);
 }
+// The same for raw MFMA results that the code behind a branch reads.
+GONN_DEV void settle_before_branch(f32x16& x, f32x16& y) {
+    asm volatile("s_nop 7\n\ts_nop 2" : "+v"(x), "+v"(y));
+}
 
 // Compile-time loop: f(std::integral_constant<int, i>) for i = 0 .. N-1.
 template <typename F, int... I>

@@ -59,6 +59,7 @@ struct Attend8 {
     int split, nsplit;         // blocks per split, splits at most
     int rows;                  // rows (heads x queries) per workgroup: 16, 32, 64 or 128
     float scale_log2;
+    float c2, sign;  // the same with the sign apart (WindowParams)
 };
 hipError_t launch_attend8(const Attend8& a, int is_bf16, hipStream_t s);
 

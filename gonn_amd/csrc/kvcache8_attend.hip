@@ -14,6 +14,8 @@
 // values are exact in bf16; a bf16 row has one product per term and its weights
 // are rounded to bf16 once, an fp32 row has q and P in three pieces. Key waves
 // merge through LDS, splits through the combine kernel.
+#include <type_traits>
+
 #include "common.h"
 #include "kvcache8.h"
 
@@ -628,16 +630,369 @@ __global__ __launch_bounds__(256, 2) void attend8_few_kernel(Attend8 a) {
     for (int t = 0; t < ND; t++) write_row4<D, T>(a, row + n, sp, t * 16 + 4 * g, oacc[t], m, lt);
 }
 
-// Splits of one row joined: one workgroup of D threads per row. A split in which
-// the row saw nothing has m = -inf and counts for nothing.
+// ---------------------------------------------------------------------------
+// Many bf16 rows (a prompt's next chunk): bound by the matrix cores, so the blocks are
+// turned to bf16 once for the workgroup's 128 rows and the three-stage pipeline of
+// window_fwd_pipe_kernel (attn_window.hip) runs on them. A thread loads its share of
+// a block (K(t+4), V(t+2)) into registers one step ahead, and in the next step's slots
+// turns it to bf16 and writes it to the two-slot LDS rings: K row-major, V transposed
+// as it lies, each 16 positions in the order of P's registers. The open block comes
+// last, straight from the ring to registers.
+// ---------------------------------------------------------------------------
+constexpr float kSumBound8 = 16384.f, kLazy8 = 8.f;
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void attend8_pipe_kernel(Attend8 a) {
+    constexpr int BM = 128, BN = 64, NKS = D / 16, NDT = D / 32, NPC = D / 64;
+    constexpr uint32_t TB = BN * D * 2;  // bytes of a K or V tile
+    constexpr int KLEAD = 3, VLEAD = 1;
+    __shared__ __attribute__((aligned(16))) bf16 sKb[2 * BN * D];
+    __shared__ __attribute__((aligned(16))) bf16 sVb[2 * BN * D];
+
+    const Cache8& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, ln = lane & 31;
+    const int T_ = a.T, R = a.Hq / c.H * T_, nrb = (R + BM - 1) / BM, BH = c.B * c.H;
+    int us, rb;
+    map_block(blockIdx.x, nrb, BH * a.nsplit, true, us, rb, 1, true);
+    const int sp = __builtin_amdgcn_readfirstlane(us / BH), bhi = us - sp * BH, b = bhi / c.H;
+    const size_t bh = bhi;
+    int len = c.len[b];
+    len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
+    const int r0 = rb * BM, r1 = r0 + BM < R ? r0 + BM : R;
+    int t0, t1;
+    query_span(r0, r1 - 1, T_, t0, t1);
+    Blocks8 bs;
+    bs.init(len - T_ + t0, len - T_ + t1, a.window, a.sinks);
+    const int nv = bs.count(), ns = splits8(a, nv);
+    if (sp >= ns && sp > 0) return;  // uniform; split 0 writes also where there is nothing to see
+    const int b0 = ns ? (int)((long long)sp * nv / ns) : 0;
+    const int b1 = ns ? (int)((long long)(sp + 1) * nv / ns) : 0;
+    const int closed = len / kBlk8;
+    const bool open = b1 > b0 && bs.block(b1 - 1) == closed;
+    const int ntiles = b1 - b0 - (open ? 1 : 0);
+
+    // This wave's rows, this lane's, and the positions that they stand for.
+    const int rw = r0 + wave * 32, ri = rw + ln, rc = ri < R ? ri : R - 1, pi = len - T_ + rc % T_;
+    int wt0 = 0, wt1 = 0;
+    if (rw < R) query_span(rw, rw + 31 < R ? rw + 31 : R - 1, T_, wt0, wt1);
+    const int pw0 = len - T_ + wt0, pw1 = len - T_ + wt1;
+    const float c2 = a.c2;
+    const bf16* qrow = (const bf16*)a.q + ((size_t)bh * R + rc) * D;
+    bf16x8 qf[NKS];
+    auto load_q = [&](int d) {  // eight channels, times the scale's sign
+        const uint32_t flip = a.sign < 0.f ? 0x80008000u : 0u, keep = a.sign != 0.f ? ~0u : 0u;
+        u32x4 x = *(const u32x4*)(qrow + d);
+        for (int e = 0; e < 4; e++) x[e] = (x[e] ^ flip) & keep;
+        return __builtin_bit_cast(bf16x8, x);
+    };
+
+    // This thread's pieces of a block, 16 codes each: keys 16 wave + lane % 16, channels
+    // 16 (lane / 16 + 4 i) ..; channels 16 (wave + 4 i) + lane % 16, positions 16 (lane /
+    // 16) ... LDS: slabs as in common.h, K of 64 rows, V^T of D.
+    const int pr = lane & 15, pc = lane >> 4;
+    u32x4 kst[NPC], vst[NPC];
+    float ksc = 1.f, vsc = 1.f;
+    auto blk_of = [&](int t) { return bs.block(b0 + (t < ntiles ? t : ntiles - 1)); };
+    const uint32_t head = (uint32_t)c.nblk * kBlk8 * D;  // bytes of a head's codes
+    const brsrc krs = make_rsrc(c.k8 + bh * head, head), vrs = make_rsrc(c.v8 + bh * head, head);
+    const uint32_t kvo = (uint32_t)((16 * wave + pr) * D + 16 * pc), vvo = (uint32_t)((16 * wave + pr) * kBlk8 + 16 * pc);
+    auto load_k = [&](int t, int i) {
+        kst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, kvo + 64 * i, blk_of(t) * kBlk8 * D, 0));
+    };
+    auto load_v = [&](int t, int i) {
+        vst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, vvo + 64 * i * kBlk8, blk_of(t) * kBlk8 * D, 0));
+    };
+    auto slot_pos = [&](int rows, int row, int chunk) {
+        return (uint32_t)((((chunk >> 2) * rows + row) * 4 + ((chunk & 3) ^ slab_swz(row))) * 16);
+    };
+    const uint32_t kp0 = slot_pos(BN, 16 * wave + pr, 2 * pc), kp1 = slot_pos(BN, 16 * wave + pr, 2 * pc + 1);
+    const uint32_t vp0 = slot_pos(D, 16 * wave + pr, 2 * pc), vp1 = slot_pos(D, 16 * wave + pr, 2 * pc + 1);
+    // Half x of piece i: eight codes to bf16 and to LDS.
+    auto put_k = [&](char* tile, int i, int x) {
+        *(bf16x8*)(tile + (x ? kp1 : kp0) + i * 2 * BN * 64) = decode8(kst[i][2 * x], kst[i][2 * x + 1], ksc);
+    };
+    auto put_v = [&](char* tile, int i, int x) {  // positions {0..3, 8..11} and {4..7, 12..15}
+        *(bf16x8*)(tile + (x ? vp1 : vp0) + i * 64 * 64) = decode8(vst[i][x], vst[i][x + 2], vsc);
+    };
+    const int hs = slab_swz(ln);
+    const uint32_t qa0 = (uint32_t)(ln * 64 + ((0 + g) ^ hs) * 16);
+    const uint32_t qa1 = (uint32_t)(ln * 64 + ((2 + g) ^ hs) * 16);
+    char *const sKc = (char*)sKb, *const sVc = (char*)sVb;
+    auto kfrag = [&](const char* tile, int ks, int mt) {
+        return *(const bf16x8*)(tile + ((ks & 1) ? qa1 : qa0) + ((ks >> 1) * BN + mt * 32) * 64);
+    };
+    auto vfrag = [&](uint32_t base, int ks, int dt) {
+        return *(const bf16x8*)(sVc + base + ((ks & 1) ? qa1 : qa0) + ((ks >> 1) * D + dt * 32) * 64);
+    };
+
+    f32x16 oacc[NDT];
+    for (int dt = 0; dt < NDT; dt++) oacc[dt] = f32x16{};
+    float mc = 0.f, l = 0.f, alpha = 1.f;
+
+    // Scores of block blk that this lane's row does not see, to -inf (c2 > 0).
+    auto mask_blk = [&](int blk, f32x16* s, auto key_of) {
+        const int kb = blk * kBlk8;
+        if (kb + 63 <= pw0 && (a.window == 0 || pw1 - kb < a.window || kb + 63 < a.sinks)) return;
+        const int hi = pi - kb, lo = a.window ? hi - a.window : -1, sk = a.sinks - kb;
+        for (int mt = 0; mt < 2; mt++)
+            for (int r = 0; r < 16; r++) {
+                const int x = key_of(mt, r);
+                s[mt][r] = x > hi || (x <= lo && x >= sk) ? -INFINITY : s[mt][r];
+            }
+    };
+    auto mask = [&](int t, f32x16* s) {
+        mask_blk(blk_of(t), s, [&](int mt, int r) { return mt * 32 + 8 * (r >> 2) + 4 * g + (r & 3); });
+    };
+    // Maximum of a tile's scaled scores over the row.
+    auto tile_max = [&](const f32x16* s) {
+        float m0 = -INFINITY;
+        for (int mt = 0; mt < 2; mt++)
+            for (int r = 0; r < 16; r++) m0 = fmaxf(m0, s[mt][r]);
+        return pair_max32(m0) * c2;
+    };
+    auto p_tile = [&](const f32x16* s, u32x4* pk) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 16; k++) {
+            const int mt = k >> 3, r = (k & 7) * 2;
+            const float x = fast_exp2(__builtin_fmaf(s[mt][r], c2, -mc));
+            const float y = fast_exp2(__builtin_fmaf(s[mt][r + 1], c2, -mc));
+            part[k & 3] += x + y;
+            const bf16x2 pr2 = {to_bf16(x), to_bf16(y)};
+            pk[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, pr2);
+        }
+        return (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    // Moves the offset to the tile's maximum where the row has seen nothing yet or the
+    // tile exceeds it by far; alpha is what that scales l and O by.
+    auto move_offset = [&](const f32x16* s) {
+        const float mx = tile_max(s);
+        const bool empty = pair_sum32(l) == 0.f;
+        const float mn = mx > -INFINITY && (empty || mx - mc > kLazy8) ? mx : mc;
+        alpha = empty ? 0.f : fast_exp2(mc - mn);
+        mc = mn;
+    };
+    u32x4 pp[4];  // P of the tile PV consumes next
+
+    // One step, scheduled by hand as in attn_window.hip. TAIL: 0 a full step; 1 the
+    // next-to-last (no S^T(t+2)); 2 the last (no P(t+1) either).
+    auto step = [&](int t, f32x16* sA, f32x16* sB, auto TAILC) __attribute__((always_inline)) {
+        constexpr int TAIL = decltype(TAILC)::value;
+        char *const ktile = sKc + ((t + KLEAD) & 1) * TB, *const vtile = sVc + ((t + VLEAD) & 1) * TB;
+        const float kn = c.ks[bh * c.nblk + blk_of(t + KLEAD + 1)], vn = c.vs[bh * c.nblk + blk_of(t + VLEAD + 1)];
+        if constexpr (TAIL < 2) mask(t + 1, sB);
+        const uint32_t vb = (uint32_t)(t & 1) * TB;
+        const char* kt = sKc + (uint32_t)(t & 1) * TB;
+
+        constexpr int SKS = NKS / 4, GW = NDT + 2 * SKS, NM = 4 * GW, NU = 16, LA = 3;
+        constexpr int NPUT = 4 * NPC, DS = NM / NPUT < 2 ? NM / NPUT : 2;  // half pieces: K's, then V's
+        static_assert(DS * NPUT <= NM, "the step's tile writes fit in its slots");
+        bf16x8 opr[4];
+        auto fetch = [&](auto E) {
+            constexpr int e = decltype(E)::value, j = e / GW, w = e % GW;
+            if constexpr (w < NDT) opr[e & 3] = vfrag(vb, j, w);
+            else if constexpr (TAIL == 0)
+                opr[e & 3] = kfrag(kt, SKS * j + ((w - NDT) >> 1), (w - NDT) & 1);
+        };
+        auto issue = [&](auto E) {
+            constexpr int e = decltype(E)::value, j = e / GW, w = e % GW;
+            if constexpr (w < NDT) {
+                oacc[w] = mfma_bf16(opr[e & 3], __builtin_bit_cast(bf16x8, pp[j]), oacc[w]);
+            } else if constexpr (TAIL == 0) {
+                constexpr int kk = SKS * j + ((w - NDT) >> 1), mt = (w - NDT) & 1;
+                sA[mt] = mfma_bf16(opr[e & 3], qf[kk], kk == 0 ? f32x16{} : sA[mt]);
+            }
+        };
+        auto put_slot = [&](auto E) {
+            constexpr int e = decltype(E)::value, d = e / DS;
+            // Tail steps write no K tile (TAIL >= 1) and no V tile (TAIL 2).
+            if constexpr (e % DS == 0 && d < NPUT && d >= (TAIL == 0 ? 0 : TAIL == 1 ? NPUT / 2 : NPUT)) {
+                constexpr int i = d % (2 * NPC) / 2, x = d % 2;
+                if constexpr (d < 2 * NPC) {
+                    put_k(ktile, i, x);
+                    if constexpr (x == 1) load_k(t + KLEAD + 1, i);
+                } else {
+                    put_v(vtile, i, x);
+                    if constexpr (x == 1) load_v(t + VLEAD + 1, i);
+                }
+            }
+        };
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        auto uslot = [](int k) { return (k >> 2) * GW + NDT + (k & 3); };
+        float ub[16][2];
+        auto uop = [&](auto U, auto S) {
+            constexpr int k = decltype(U)::value, stage = decltype(S)::value;
+            constexpr int mt = k >> 3, r = (k & 7) * 2;
+            if constexpr (stage == 0) {
+                ub[k][0] = fast_exp2(__builtin_fmaf(sB[mt][r], c2, -mc));
+                ub[k][1] = fast_exp2(__builtin_fmaf(sB[mt][r + 1], c2, -mc));
+                pin(ub[k][0]);
+                pin(ub[k][1]);
+            } else {
+                part[k & 3] += ub[k][0] + ub[k][1];
+                const bf16x2 pr = {to_bf16(ub[k][0]), to_bf16(ub[k][1])};
+                pp[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, pr);
+                pin(pp[k >> 2][k & 3]);
+                pin(part[k & 3]);
+            }
+        };
+        auto uops_at = [&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (TAIL == 2) return;
+            static_for<2>([&](auto S) {
+                static_for<NU>([&](auto U) {
+                    constexpr int at = uslot(decltype(U)::value) - 2 + 2 * decltype(S)::value;
+                    if constexpr (e < NM ? at == e : at >= NM) uop(U, S);
+                });
+            });
+        };
+        __builtin_amdgcn_s_setprio(1);
+        static_for<LA>([&](auto E) { fetch(E); });
+        static_for<NM>([&](auto E) {
+            constexpr int e = decltype(E)::value;
+            if constexpr (e + LA < NM) fetch(std::integral_constant<int, e + LA>{});
+            issue(E);
+            put_slot(E);
+            uops_at(E);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        uops_at(std::integral_constant<int, NM>{});
+        __builtin_amdgcn_s_setprio(0);
+        float ts = (part[0] + part[1]) + (part[2] + part[3]);
+        alpha = 1.f;
+        if (TAIL < 2 && __builtin_amdgcn_ballot_w64(!(ts <= kSumBound8) || l == 0.f)) {
+            move_offset(sB);
+            ts = p_tile(sB, pp);
+        }
+        l = l * alpha + ts;
+        ksc = kn;
+        vsc = vn;
+        __syncthreads();
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.f))
+            for (int dt = 0; dt < NDT; dt++) oacc[dt] *= alpha;
+    };
+
+    if (ntiles > 0) {
+        // Prologue: S^T(0) -> P(0), S^T(1); K(0) is staged in V slot 1.
+        f32x16 s0[2], s1[2];
+        auto qk_tile = [&](const char* tile, f32x16* s) {
+            s[0] = s[1] = f32x16{};
+            for (int ks = 0; ks < NKS; ks++)
+                for (int mt = 0; mt < 2; mt++) s[mt] = mfma_bf16(kfrag(tile, ks, mt), qf[ks], s[mt]);
+        };
+        auto fill_k = [&](int t, char* tile) {
+            ksc = c.ks[bh * c.nblk + blk_of(t)];
+            for (int i = 0; i < NPC; i++) load_k(t, i);
+            for (int i = 0; i < NPC; i++)
+                for (int x = 0; x < 2; x++) put_k(tile, i, x);
+        };
+        fill_k(0, sVc + TB);
+        fill_k(1, sKc + TB);
+        fill_k(2, sKc);
+        vsc = c.vs[bh * c.nblk + blk_of(0)];
+        for (int i = 0; i < NPC; i++) load_v(0, i);
+        for (int i = 0; i < NPC; i++)
+            for (int x = 0; x < 2; x++) put_v(sVc, i, x);
+        for (int i = 0; i < NPC; i++) {  // what step 0 puts
+            load_k(KLEAD, i);
+            load_v(VLEAD, i);
+        }
+        ksc = c.ks[bh * c.nblk + blk_of(KLEAD)];
+        vsc = c.vs[bh * c.nblk + blk_of(VLEAD)];
+        for (int ks = 0; ks < NKS; ks++) qf[ks] = load_q(ks * 16 + g * 8);
+        __syncthreads();
+        qk_tile(sVc + TB, s0);
+        qk_tile(sKc + TB, s1);
+        settle_before_branch(s0[0], s0[1]);
+        settle_before_branch(s1[0], s1[1]);
+        mask(0, s0);
+        mc = tile_max(s0);
+        if (!(mc > -INFINITY)) mc = 0.f;  // nothing seen yet: no offset
+        l = p_tile(s0, pp);
+        __syncthreads();  // K(0) and K(1) read by every wave
+
+        const std::integral_constant<int, 0> full;
+        const std::integral_constant<int, 1> tail1;
+        const std::integral_constant<int, 2> tail2;
+        const int nfull = ntiles - 2;
+        int t = 0;
+        for (; t + 1 < nfull; t += 2) {
+            step(t, s0, s1, full);
+            step(t + 1, s1, s0, full);
+        }
+        if (t < nfull) step(t++, s0, s1, full);
+        if (ntiles >= 2) {
+            if (t & 1)
+                for (int mt = 0; mt < 2; mt++) {
+                    const f32x16 x = s0[mt];
+                    s0[mt] = s1[mt];
+                    s1[mt] = x;
+                }
+            step(t, s0, s1, tail1);
+        }
+        step(ntiles - 1, s1, s0, tail2);
+    }
+    if (open && rw < R) {
+        // The open block, bf16, with the operands of attend8_kernel: register r of tile u
+        // is position 32 u + 16 g + r. Positions past the last are no one's values.
+        const int krow = 16 * ((ln >> 2) & 1) + 4 * (ln >> 3) + (ln & 3), n = len - closed * kBlk8;
+        const uint16_t* kp = c.kt + ((bh * 2 + (closed & 1)) * kBlk8 + krow) * D + 16 * g;
+        const uint16_t* vp = c.vt + ((bh * 2 + (closed & 1)) * D + ln) * kBlk8 + 16 * g;
+        f32x16 s[2];
+        s[0] = s[1] = f32x16{};
+        for (int u = 0; u < 2; u++)
+            for (int j = 0; j < D / 32; j++)
+                for (int x = 0; x < 2; x++)
+                    s[u] = mfma_bf16(*(const bf16x8*)(kp + u * 32 * D + 32 * j + 8 * x),
+                                     load_q(32 * j + 16 * g + 8 * x), s[u]);
+        settle_before_branch(s[0], s[1]);
+        mask_blk(closed, s, [&](int u, int r) { return 32 * u + 16 * g + r; });
+        alpha = 1.f;
+        move_offset(s);
+        const float ts = p_tile(s, pp);
+        l = l * alpha + ts;
+        for (int t = 0; t < NDT; t++) {
+            oacc[t] *= alpha;
+            for (int u = 0; u < 2; u++)
+                for (int x = 0; x < 2; x++) {
+                    u16x8 v = *(const u16x8*)(vp + (size_t)t * 32 * kBlk8 + 32 * u + 8 * x);
+                    for (int e = 0; e < 8; e++) v[e] = 32 * u + 16 * g + 8 * x + e < n ? v[e] : (uint16_t)0;
+                    oacc[t] = mfma_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pp[2 * u + x]), oacc[t]);
+                }
+        }
+    }
+
+    const float lt = pair_sum32(l);
+    bool bad = nonfinite(lt);
+    for (int t = 0; t < NDT; t++)
+        for (int r = 0; r < 16; r++) bad |= nonfinite(oacc[t][r]);
+    const size_t row = (size_t)bh * R + ri;
+    if (__builtin_amdgcn_ballot_w64(bad && ri < R)) {
+        attend8_plain<D>(a, bh, len, qrow, bs, b0, b1, pi, row, sp, ri < R);
+        return;
+    }
+    if (ri >= R) return;
+    // A row that saw nothing has no offset (its share of a combine is nothing).
+    const float m = lt == 0.f ? -INFINITY : mc;
+    for (int t = 0; t < NDT; t++)
+        for (int rq = 0; rq < 4; rq++)
+            write_row4<D, bf16>(a, row, sp, t * 32 + rq * 8 + g * 4,
+                                f32x4{oacc[t][rq * 4], oacc[t][rq * 4 + 1], oacc[t][rq * 4 + 2], oacc[t][rq * 4 + 3]},
+                                m, lt);
+}
+
+// Splits joined: a thread takes four channels of a row, 16 bytes of each split (a
+// workgroup per row took 31 us for 32768 rows of 4 splits). A split in which the row
+// saw nothing has m = -inf and counts for nothing.
 template <int D, typename T>
-__global__ __launch_bounds__(D) void attend8_combine_kernel(Attend8 a) {
-    const size_t row = blockIdx.x;
-    const int R = a.Hq / a.c.H * a.T, tid = threadIdx.x;
-    const int bh = (int)(row / R), r = (int)(row - (size_t)bh * R);
+__global__ __launch_bounds__(256) void attend8_combine_kernel(Attend8 a, unsigned rows) {
+    const unsigned row = (blockIdx.x * 256 + threadIdx.x) / (D / 4);
+    if (row >= rows) return;
+    const int d = threadIdx.x % (D / 4) * 4, R = a.Hq / a.c.H * a.T;
+    const int bh = (int)(row / (unsigned)R), r = (int)(row - (unsigned)bh * R);
     int len = a.c.len[bh / a.c.H];
     len = len < a.c.Lmax ? len : a.c.Lmax;
-    // The row's workgroup and its splits, as the kernel above cuts them.
+    // The row's workgroup and its splits, as the kernels above cut them.
     const int r0 = r / a.rows * a.rows, r1 = r0 + a.rows < R ? r0 + a.rows : R;
     int t0, t1;
     query_span(r0, r1 - 1, a.T, t0, t1);
@@ -645,19 +1000,27 @@ __global__ __launch_bounds__(D) void attend8_combine_kernel(Attend8 a) {
     bs.init(len - a.T + t0, len - a.T + t1, a.window, a.sinks);
     int ns = splits8(a, bs.count());
     ns = ns < 1 ? 1 : ns;
-    const float* ml = a.part_ml + row * a.nsplit * 2;
-    const float* po = a.part_o + row * a.nsplit * D;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2* ml = (const f32x2*)a.part_ml + (size_t)row * a.nsplit;
+    const float* po = a.part_o + (size_t)row * a.nsplit * D + d;
     float M = -INFINITY;
-    for (int i = 0; i < ns; i++) M = fmaxf(M, ml[2 * i]);
-    float L = 0.f, O = 0.f;
+    for (int i = 0; i < ns; i++) M = fmaxf(M, ml[i][0]);
+    float L = 0.f;
+    f32x4 O = f32x4{};
     for (int i = 0; i < ns; i++) {
-        const float w = ml[2 * i] == -INFINITY ? 0.f : fast_exp2(ml[2 * i] - M);
-        L = __builtin_fmaf(w, ml[2 * i + 1], L);
-        O = __builtin_fmaf(w, po[(size_t)i * D + tid], O);
+        const f32x2 x = ml[i];
+        const float w = x[0] == -INFINITY ? 0.f : fast_exp2(x[0] - M);
+        L = __builtin_fmaf(w, x[1], L);
+        const f32x4 v = *(const f32x4*)(po + (size_t)i * D);
+        for (int e = 0; e < 4; e++) O[e] = __builtin_fmaf(w, v[e], O[e]);
     }
-    const float o = L == 0.f ? 0.f : O / L;
-    if constexpr (sizeof(T) == 4) ((float*)a.o)[row * D + tid] = o;
-    else ((bf16*)a.o)[row * D + tid] = to_bf16(o);
+    for (int e = 0; e < 4; e++) O[e] = L == 0.f ? 0.f : O[e] / L;
+    if constexpr (sizeof(T) == 4) *(f32x4*)((float*)a.o + (size_t)row * D + d) = O;
+    else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        *(bf16x4*)((bf16*)a.o + (size_t)row * D + d) =
+            bf16x4{to_bf16(O[0]), to_bf16(O[1]), to_bf16(O[2]), to_bf16(O[3])};
+    }
 }
 
 namespace {
@@ -669,9 +1032,12 @@ void run_attend8(const Attend8& a, hipStream_t s) {
     const unsigned grid = (unsigned)((R + a.rows - 1) / a.rows) * (unsigned)(a.c.B * a.c.H) * (unsigned)a.nsplit;
     if (a.rows == 16) attend8_few_kernel<D, T><<<grid, 256, 0, s>>>(a);
     else if (a.rows == 32) attend8_kernel<D, T, 1><<<grid, 256, 0, s>>>(a);
-    else if (a.rows == 64) attend8_kernel<D, T, 2><<<grid, 256, 0, s>>>(a);
+    else if (a.rows == 128 && sizeof(T) == 2 && (double)a.c.nblk * kBlk8 * D < 4.0e9) {  // 32-bit offsets
+        if constexpr (sizeof(T) == 2) attend8_pipe_kernel<D><<<grid, 256, 0, s>>>(a);
+    } else if (a.rows == 64) attend8_kernel<D, T, 2><<<grid, 256, 0, s>>>(a);
     else attend8_kernel<D, T, 4><<<grid, 256, 0, s>>>(a);
-    if (a.nsplit > 1) attend8_combine_kernel<D, T><<<rows, D, 0, s>>>(a);
+    if (a.nsplit > 1)
+        attend8_combine_kernel<D, T><<<(rows + 1024 / D - 1) / (1024 / D), 256, 0, s>>>(a, rows);
 }
 
 }  // namespace
