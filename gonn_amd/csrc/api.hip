@@ -861,8 +861,12 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     // long ones stream faster (2048 heads of 8192 positions, D 128: 16 blocks 5.4
     // TB/s, 32 6.2, 64 6.6, 128 6.9), but sequences of different lengths level out
     // less (512 to 8192: 441, 397, 387, 390 us). Shorter ones where the device has
-    // room for more workgroups, down to a block per key wave.
-    const long long want = (p.rows == 128 ? 2 : 4) * cus, least = p.rows <= 32 ? 4 : 128 / p.rows;
+    // room for more workgroups, down to two blocks per key wave; but no more than one
+    // split for up to 24 blocks, which spares the second kernel (8 heads, D 128, 16
+    // blocks 11 us against 16, replayed 11 against 12; 32 blocks 16 and 16, replayed
+    // 16 and 12; 64 blocks in splits of 4, 8 and 16: 16, 14, 15 us replayed).
+    const long long want = (p.rows == 128 ? 2 : 4) * cus;
+    const long long least = p.rows <= 32 ? (blocks <= 24 ? blocks : 8) : 128 / p.rows;
     long long split = 64;
     if (units * ((blocks + split - 1) / split) < want)
         split = std::min(split, std::max(least, blocks * units / want));
