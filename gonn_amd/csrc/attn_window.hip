@@ -549,8 +549,16 @@ void pick_window_fwd(const WindowParams& p, hipStream_t s) {
         else if (b64 >= cus) run_window_fwd<D, T, 2, 2, 2>(p, s);
         else run_window_fwd<D, T, 1, 2, 1>(p, s);
     } else {
-        if (b128 >= 2 * cus) run_window_fwd<D, T, 4, 1, 2>(p, s);
-        else run_window_fwd<D, T, 2, 1, 1>(p, s);
+        // fp32, us: B 8, H 12, S 1024, window 256, D 64: 128 rows 57, 64 rows 73; 4 x 12 x
+        // 1021, window 200: 40 and 41; 8 heads x 1000: 30 and 19; D 128: 4 x 16 over 8,
+        // 2048, window 512: 217 and 346; 8 x 1000: 47 and 32.
+        if constexpr (D == 64) {
+            if (b128 >= cus) run_window_fwd<D, T, 4, 2, 3>(p, s);
+            else run_window_fwd<D, T, 2, 1, 2>(p, s);
+        } else {
+            if (b128 >= cus) run_window_fwd<D, T, 4, 1, 2>(p, s);
+            else run_window_fwd<D, T, 2, 1, 1>(p, s);
+        }
     }
 }
 

@@ -856,6 +856,10 @@ DkdvShape dkdv_shape(const WindowParams& p, int D, int is_bf16) {
     // The 128-key kernel reads a key head's queries with 32-bit offsets.
     const bool near = (double)(p.H / p.Hkv) * p.Sp * D * 2 < 4.0e9;
     if (b128 >= cus && is_bf16 && near) return {128, 64};
+    // fp32, us: D 64 64 keys and two waves per SIMD (the sizes of the forward's note: 99;
+    // 61; 25; one wave 147; 78; 25; 128 keys 104; -; 25). D 128: 128 keys 560; 44, 64
+    // keys 671; 49.
+    if (!is_bf16 && D == 128) return {128, 32};
     return {64, 64};
 }
 
@@ -864,9 +868,9 @@ void run_dkdv(const WindowParams& p, int BK, int BQ, hipStream_t s) {
     const unsigned grid = (unsigned)p.slots * (unsigned)(p.B * p.Hkv);
     if constexpr (sizeof(T) == 2) {
         if (BK == 128) window_dkdv_pipe_kernel<D><<<grid, 256, 0, s>>>(p);
-        else window_dkdv_kernel<D, T, 2, 2, 1><<<grid, 256, 0, s>>>(p);
+        else window_dkdv_kernel<D, T, 2, 2, D == 64 ? 2 : 1><<<grid, 256, 0, s>>>(p);
     } else {
-        window_dkdv_kernel<D, T, 2, 1, 1><<<grid, 256, 0, s>>>(p);
+        window_dkdv_kernel<D, T, D == 64 ? 2 : 4, 1, D == 64 ? 2 : 1><<<grid, 256, 0, s>>>(p);
     }
     if (p.per_tail)
         window_dkdv_kernel<D, T, tail_keys(D, sizeof(T) == 4) / 32, sizeof(T) == 2 ? 2 : 1, 1, true>
@@ -886,9 +890,17 @@ void run_window_bwd(const WindowParams& p, hipStream_t s) {
     const DkdvShape sh = dkdv_shape(p, D, sizeof(T) == 2);
     if constexpr (sizeof(T) == 2) {
         if (b128 >= 2 * cus) window_dq_kernel<D, T, 4, 2, 2><<<g128, 256, 0, s>>>(p);
-        else window_dq_kernel<D, T, 2, 2, 1><<<g64, 256, 0, s>>>(p);
+        else window_dq_kernel<D, T, 2, 2, 2><<<g64, 256, 0, s>>>(p);
     } else {
-        window_dq_kernel<D, T, 2, 1, 1><<<g64, 256, 0, s>>>(p);
+        // fp32, us, 128 and 64 rows: D 64, the forward's sizes: 91, 87; 50, 55; 36, 25; 2 x
+        // 16 x 4096, window 1024: 277, 292. D 128: 439, 494; 67, 45.
+        if constexpr (D == 64) {
+            if (b128 >= cus) window_dq_kernel<D, T, 4, 2, 2><<<g128, 256, 0, s>>>(p);
+            else window_dq_kernel<D, T, 2, 1, 2><<<g64, 256, 0, s>>>(p);
+        } else {
+            if (b128 >= cus) window_dq_kernel<D, T, 4, 2, 1><<<g128, 256, 0, s>>>(p);
+            else window_dq_kernel<D, T, 2, 1, 1><<<g64, 256, 0, s>>>(p);
+        }
     }
     run_dkdv<D, T>(p, sh.BK, sh.BQ, s);
 }
@@ -903,12 +915,14 @@ WindowParts plan_window_bwd(WindowParams& p, int D, int is_bf16) {
     const long long stages = ((long long)sh.BK - 1 + p.window + sh.BQ - 1) / sh.BQ;
     const long long band = std::min<long long>(all, G * (stages + 1));
     // Sinks are read by every later query. Up to 32 of them (one tile) have those
-    // queries in items of 32 keys and four waves along the queries; with more, their
-    // blocks have all queries and more items.
+    // queries in items of 32 keys and four waves along the queries, in a kernel of its
+    // own, where that takes many steps off the first one (its 15 us pay from 4 to 8
+    // steps per CU on); else their blocks have all queries and more items.
     const long long tail_q0 = stages * sh.BQ;
     p.per_tail = 0;
     p.sink_blocks = std::min(nkb, (p.sinks + sh.BK - 1) / sh.BK);
-    if (p.sinks > 0 && p.sinks <= 32 && tail_q0 < p.Sq) {
+    if (p.sinks > 0 && p.sinks <= 32 && tail_q0 < p.Sq &&
+        slices * (all - band) >= (is_bf16 ? 4 : 2) * want) {
         p.sink_blocks = 0;
         p.tail_q0 = (int)tail_q0;
         const int rows = tail_rows(D, !is_bf16);
@@ -916,11 +930,13 @@ WindowParts plan_window_bwd(WindowParams& p, int D, int is_bf16) {
         p.tail_chunk = (int)std::max<long long>(2, (steps * slices + want / 2 - 1) / (want / 2));
         p.per_tail = (int)((steps + p.tail_chunk - 1) / p.tail_chunk);
     }
-    // Items as long as a block's band, shorter where that leaves the device
-    // without work, but no shorter than 4 stages.
-    const long long items = slices * nkb;
+    // Items as long as a block's band, shorter where that leaves workgroup slots (one
+    // per CU with 128 bf16 keys, else two) without work, but no shorter than two
+    // stages: the sum of the partials costs 4 to 15 us (8 heads over 2, 777, D 128: two
+    // stages 19 + 5 us, four 22 + 4, eight 31 + 4).
+    const long long items = slices * nkb, fill = is_bf16 && sh.BK == 128 ? want / 2 : want;
     long long chunk = band;
-    if (items < want) chunk = std::max<long long>(4, (band * items + want - 1) / want);
+    if (items < fill) chunk = std::max<long long>(2, (band * items + fill - 1) / fill);
     chunk = std::min(chunk, all);
     p.chunk = (int)chunk;
     p.per_block = (int)((band + chunk - 1) / chunk);

@@ -5,15 +5,15 @@ import math
 import torch
 
 
-def sees(Sq, Sk, window, sinks, kv_len=None):
+def sees(Sq, Sk, window, sinks, kv_len=None, device="cpu"):
     """(B or 1, 1, Sq, Sk)"""
-    i, j = torch.arange(Sq)[:, None], torch.arange(Sk)[None, :]
+    i, j = torch.arange(Sq, device=device)[:, None], torch.arange(Sk, device=device)[None, :]
     m = ((j <= i) & ((i - j < window) | (j < sinks)))[None, None]
-    return m if kv_len is None else m & (j < torch.tensor(kv_len)[:, None, None, None])
+    return m if kv_len is None else m & (j < torch.tensor(kv_len, device=device)[:, None, None, None])
 
 
 def _masked(x, m):
-    return torch.where(m, x, torch.zeros((), dtype=x.dtype))
+    return torch.where(m, x, torch.zeros((), dtype=x.dtype, device=x.device))
 
 
 def _mm(p, x, m):
@@ -26,27 +26,27 @@ def _mm(p, x, m):
     return out
 
 
-def fwd(q, k, v, scale, window, sinks, kv_len=None):
+def fwd(q, k, v, scale, window, sinks, kv_len=None, device="cpu"):
     """o, lse, and sum_j p |v|."""
-    q, k, v = (x.detach().cpu().double() for x in (q, k, v))
+    q, k, v = (x.detach().to(device).double() for x in (q, k, v))
     G = q.shape[1] // k.shape[1]
     k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
-    m = sees(q.shape[2], k.shape[2], window, sinks, kv_len).expand(q.shape[0], q.shape[1], -1, -1)
+    m = sees(q.shape[2], k.shape[2], window, sinks, kv_len, device).expand(q.shape[0], q.shape[1], -1, -1)
     s = (q @ k.transpose(-1, -2) * scale).masked_fill(~m, -math.inf)
     lse = torch.logsumexp(s, -1)
     p = _masked(torch.exp(s - torch.where(torch.isinf(lse) & (lse < 0), torch.zeros_like(lse), lse)[..., None]), m)
     return _mm(p, v, m), lse, _mm(p, v.abs(), m)
 
 
-def bwd(q, k, v, o, lse, dO, scale, window, sinks, kv_len=None):
+def bwd(q, k, v, o, lse, dO, scale, window, sinks, kv_len=None, device="cpu"):
     """(dq, dk, dv), their absolute sums, and the sums with |dO| |v| + |dO| |o| in the place of
     |dS / P|: the difference dP - delta keeps the roundings of both, however small it is."""
-    q, k, v, o, lse, dO = (x.detach().cpu().double() for x in (q, k, v, o, lse, dO))
+    q, k, v, o, lse, dO = (x.detach().to(device).double() for x in (q, k, v, o, lse, dO))
     B, H, Sq, D = q.shape
     Hkv, Sk = k.shape[1:3]
     G = H // Hkv
     kh, vh = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)
-    m = sees(Sq, Sk, window, sinks, kv_len).expand(B, H, -1, -1)
+    m = sees(Sq, Sk, window, sinks, kv_len, device).expand(B, H, -1, -1)
     mt = m.transpose(-1, -2)
     lse = lse.view(B, H, Sq, 1)
     s = (q @ kh.transpose(-1, -2) * scale).masked_fill(~m, -math.inf)
@@ -71,6 +71,8 @@ def check(got, ref, total, what, noise=None):
     at most 2^-24 of the products' absolute sum: under 2^-18 of it together. A query that
     sees one key has dS = 0 and nothing but that."""
     g = got.detach().cpu().double()
+    ref, total = ref.cpu(), total.cpu()
+    noise = noise if noise is None else noise.cpu()
     assert g.shape == ref.shape, what
     assert torch.equal(torch.isnan(g), torch.isnan(ref)), f"{what}: NaN in other places"
     ok = torch.isfinite(ref)

@@ -73,6 +73,29 @@ def test_forward_and_backward(c, dtype):
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("c", [(1, 32, 32, 4500, 4500, 64, 70, 4, None), (2, 32, 16, 2700, 2690, 128, 40, 32, (2690, 31))],
+                         ids=lambda c: "x".join(map(str, c[:8])))
+def test_long_sequences_with_sinks(c, dtype):
+    """So many later queries of the sinks that they have items of their own. The reference
+    in 64 bits on the GPU."""
+    from gonn_amd import hip
+    window, sinks, kv = c[6:]
+    q, k, v, dO = _data(c, dtype, 13)
+    scale = 1.0 / math.sqrt(c[5])
+    o, lse = hip.attn_window_fwd(q, k, v, window=window, sinks=sinks, kv_len=_len(kv))
+    ro, rl, ra = ref.fwd(q, k, v, scale, window, sinks, kv, "cuda")
+    ref.check(o, ro, ra, f"o {c}")
+    _check_lse(lse, rl.cpu(), c)
+    del ro, rl, ra
+    grads = hip.attn_window_bwd(q, k, v, o, lse, dO, window=window, sinks=sinks, kv_len=_len(kv))
+    rg, rs, rn = ref.bwd(q, k, v, o, lse, dO, scale, window, sinks, kv, "cuda")
+    for name, g, r, s, n in zip(("dq", "dk", "dv"), grads, rg, rs, rn):
+        ref.check(g, r, s, f"{name} {c}", n)
+    again = hip.attn_window_bwd(q, k, v, o, lse, dO, window=window, sinks=sinks, kv_len=_len(kv))
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
 def test_gradients_against_differences():
     """Central differences of sum(O dO) in fp32: step 2^-6, whose own error is of order
     step^2 = 2^-12 of the third derivative and 2^-24 / step of the sum's rounding."""
