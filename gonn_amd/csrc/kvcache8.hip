@@ -4,10 +4,9 @@
 // closes the block when they complete it: the 64 rows (older ones from the ring)
 // go to LDS, K's and V's largest magnitudes give the scales, the codes are written
 // as they lie (K) and transposed (V). Rows of the last two blocks also go to the
-// ring. A call of more than 64 rows writes the ring in a second launch, since a
-// later block's rows would otherwise overwrite the half that the first block's
-// workgroup still reads. A sequence's length is advanced on the device by the last
-// of its workgroups, so a captured append can be replayed.
+// ring; those of the half that the first block's workgroup reads are written by that
+// workgroup, behind its reads. A sequence's length is advanced on the device by the
+// last of its workgroups, so a captured append can be replayed.
 //
 // All of it is bound by memory.
 #include "common.h"
@@ -56,14 +55,13 @@ GONN_DEV float wave_max(float x) {
 
 }  // namespace
 
-// QUANT: close blocks; RING: write the ring and advance the lengths.
-template <int D, typename T, bool QUANT, bool RING>
+template <int D, typename T>
 __global__ __launch_bounds__(256) void append8_kernel(Cache8 c, const T* __restrict__ ksrc,
                                                       const T* __restrict__ vsrc, int T_, int nb,
                                                       Seqs8 cnt) {
     constexpr int CPR = D / 8, NCH = kBlk8 * CPR, PT = NCH / 256;  // 8-element chunks
     constexpr int VS = kBlk8 + 4;  // row stride of the transposed tile, in elements
-    __shared__ __attribute__((aligned(16))) uint16_t vtile[QUANT || RING ? D * VS : 1];
+    __shared__ __attribute__((aligned(16))) uint16_t vtile[D * VS];
     __shared__ float red[2][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i = blockIdx.x % nb, u = blockIdx.x / nb, bi = u / c.H, h = u - bi * c.H;
@@ -72,12 +70,17 @@ __global__ __launch_bounds__(256) void append8_kernel(Cache8 c, const T* __restr
     const int pos = c.len[b];
     int n = seq_number(cnt, bi);
     n = pos + n <= c.Lmax ? n : 0;  // the host refuses such calls; a replayed graph may get here
-    // Without QUANT: the two blocks that the ring holds afterwards.
-    const int end = pos + n, blk = (QUANT ? pos / kBlk8 : end / kBlk8 - 1) + i, base = blk * kBlk8;
-    const int p0 = pos > base ? pos : base, p1 = end < base + kBlk8 ? end : base + kBlk8;
-    if (p0 < p1) {  // uniform
-        const bool closing = QUANT && end >= base + kBlk8;
-        const bool keep = RING && blk >= end / kBlk8 - 1;
+    const int end = pos + n, first = pos / kBlk8, open = end / kBlk8;
+    // Blocks first + i, and in the first one's workgroup the later block that takes its
+    // half of the ring (the open one or the one before it), for its ring rows only.
+    const int other = open - ((open ^ first) & 1);
+    for (int pass = 0; pass < (i == 0 && other > first ? 2 : 1); pass++) {
+        const int blk = pass ? other : first + i, base = blk * kBlk8;
+        const int p0 = pos > base ? pos : base, p1 = end < base + kBlk8 ? end : base + kBlk8;
+        if (p0 >= p1) continue;  // uniform
+        const bool closing = !pass && end >= base + kBlk8;
+        const bool keep = blk >= open - 1 && (pass || blk == first || ((blk ^ first) & 1));
+        __syncthreads();  // the LDS tile is free
         uint16_t* kring = c.kt + (bh * 2 + (blk & 1)) * kBlk8 * D;
         uint16_t* vring = c.vt + (bh * 2 + (blk & 1)) * D * kBlk8;
         u16x8 kx[PT];
@@ -165,19 +168,15 @@ __global__ __launch_bounds__(256) void append8_kernel(Cache8 c, const T* __restr
             }
         }
     }
-    if constexpr (RING) {
-        // The length was read above (the branches waited for it); the last of the
-        // sequence's workgroups to say so advances it. One counter, and one cache
-        // line, per sequence: updates of one address take about 40 ns each, 2048 on
-        // one 84 us.
-        __syncthreads();
-        unsigned* ticket = c.ticket + (size_t)b * kTicketStep8;
-        if (tid == 0 && atomicAdd(ticket, 1u) == (unsigned)(c.H * nb) - 1) {
-            const int first = (end / kBlk8 - 1) * kBlk8;
-            c.len[b] = end;
-            if (first > c.lo[b]) c.lo[b] = first;
-            *ticket = 0;
-        }
+    // The length was read above (the branches waited for it); the last of the
+    // sequence's workgroups to say so advances it. One counter, and one cache line,
+    // per sequence: updates of one address take about 40 ns each, 2048 on one 84 us.
+    __syncthreads();
+    unsigned* ticket = c.ticket + (size_t)b * kTicketStep8;
+    if (tid == 0 && atomicAdd(ticket, 1u) == (unsigned)(c.H * nb) - 1) {
+        c.len[b] = end;
+        if ((open - 1) * kBlk8 > c.lo[b]) c.lo[b] = (open - 1) * kBlk8;
+        *ticket = 0;
     }
 }
 
@@ -267,14 +266,7 @@ void run_append8(const Cache8& c, const void* k, const void* v, int rows, const 
                  hipStream_t s) {
     const int nb = (rows + 2 * kBlk8 - 2) / kBlk8;  // blocks that `rows` positions can touch
     const unsigned grid = (unsigned)cnt.nb * (unsigned)c.H * (unsigned)nb;
-    const T *ks = (const T*)k, *vs = (const T*)v;
-    if (rows <= kBlk8) {
-        append8_kernel<D, T, true, true><<<grid, 256, 0, s>>>(c, ks, vs, rows, nb, cnt);
-    } else {
-        append8_kernel<D, T, true, false><<<grid, 256, 0, s>>>(c, ks, vs, rows, nb, cnt);
-        append8_kernel<D, T, false, true>
-            <<<(unsigned)cnt.nb * (unsigned)c.H * 2u, 256, 0, s>>>(c, ks, vs, rows, 2, cnt);
-    }
+    append8_kernel<D, T><<<grid, 256, 0, s>>>(c, (const T*)k, (const T*)v, rows, nb, cnt);
 }
 
 }  // namespace
