@@ -477,6 +477,18 @@ def attn_decode(q, kcache, vcache, kv_len, *, scale=None, split_keys: int = 0, o
     return out
 
 
+def _call_workspace(nbytes, device, stream):
+    """Workspace of one call on the current stream (`stream`: it, where known). Inside a
+    graph capture each call has its own, from the graph's pool: the shared one may grow
+    (and move) later, and two graphs that share it could not run side by side."""
+    if nbytes == 0:
+        return None
+    torch = _torch()
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    return _WS.get(nbytes, device, stream)
+
+
 class _OnStream:
     """A call's device and stream, with the call's allocations on that stream;
     tensors used on a stream other than the current one are marked as used there,
@@ -517,15 +529,19 @@ class _OnStream:
             c.__exit__(*exc)
 
     def workspace(self, nbytes):
-        """Workspace of one call. Inside a graph capture each call has its own,
-        from the graph's pool: the shared one may grow (and move) later, and two
-        graphs that share it could not run side by side."""
-        if nbytes == 0:
-            return None
-        torch = _torch()
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(int(nbytes), dtype=torch.uint8, device=self.device)
-        return _WS.get(nbytes, self.device, self._stream)
+        return _call_workspace(nbytes, self.device, self._stream)
+
+
+def _plain_stream(device, stream, tensors):
+    """The raw stream of a call on the current device and stream whose tensors all lie
+    on that device (nothing to switch, nothing to mark), else None."""
+    torch = _torch()
+    if stream is not None or device.type != "cuda" or device.index != torch.cuda.current_device():
+        return None
+    for x in tensors:
+        if x is not None and x.device != device:
+            return None  # _OnStream names them
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _window_shapes(what, q, k, v):
@@ -566,7 +582,7 @@ def attn_window_fwd(q, k, v, *, window: int, sinks: int = 0, scale=None, kv_len=
         else:
             _window_like("attn_window_fwd", "out", out, q)
         if lse_out is None and lse:
-            lse_out = torch.empty((B * H, Sq), dtype=torch.float32, device=q.device)
+            lse_out = q.new_empty((B * H, Sq), dtype=torch.float32)
         a = WindowFwdArgs(buf(q), buf(k), buf(v), buf(out), buf(lse_out), B, H, Hkv, Sq, Sk, D,
                           float(scale), int(window), int(sinks), buf(kv_len))
         check(_lib.load().gonn_hip_attn_window_fwd(ctypes.byref(a), None, 0, on.ptr),
@@ -757,7 +773,10 @@ class KVCache8:
         self._h = ctypes.c_void_p()
         check(_lib.load().gonn_hip_kvcache8_create(ctypes.byref(self._h), self.B, self.H,
                                                    self.Lmax, self.D), "KVCache8")
-        self.device = _torch().device("cuda", _torch().cuda.current_device())
+        torch = _torch()
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._int_array = ctypes.c_int * self.B
+        self._bf16 = torch.empty(0, dtype=torch.bfloat16, device=self.device)
 
     def close(self) -> None:
         if self._h:
@@ -785,41 +804,50 @@ class KVCache8:
         return _OnStream(self.device, stream, tensors)
 
     def _ints(self, n, what):
-        a = np.ascontiguousarray(n, dtype=np.int32)
-        if a.shape != (self.B,):
+        """B whole numbers as a C array."""
+        if isinstance(n, np.ndarray):
+            if n.dtype.kind not in "iu":
+                raise TypeError(f"KVCache8: {what} must be whole numbers")
+            n = n.tolist()
+        if len(n) != self.B:
             raise ValueError(f"KVCache8: {what} must have {self.B} entries")
-        return a, a.ctypes.data_as(ctypes.POINTER(ctypes.c_int))
+        return self._int_array(*n)
+
+    def _run(self, what, call, stream, *tensors):
+        """call(raw stream) on the call's stream."""
+        st = _plain_stream(self.device, stream, tensors)
+        if st is not None:
+            check(call(st), what)
+            return
+        with self._on(stream, *tensors) as on:
+            check(call(on.ptr), what)
 
     def lengths(self, stream=None) -> np.ndarray:
-        out, p = self._ints(np.zeros(self.B), "lengths")
-        with self._on(stream) as on:
-            check(_lib.load().gonn_hip_kvcache8_lengths(self._live(), p, on.ptr), "KVCache8.lengths")
-        return out
+        out, h, lib = self._int_array(), self._live(), _lib.load()
+        self._run("KVCache8.lengths", lambda st: lib.gonn_hip_kvcache8_lengths(h, out, st), stream)
+        return np.array(out, dtype=np.int32)
 
     def append(self, k, v, counts=None, stream=None) -> None:
         """k, v device (B,H,T,D) float32 or bfloat16 (both the same); sequence b takes
         its first counts[b] rows (host numbers; all T when None)."""
-        if k.dim() != 4 or tuple(k.shape) != tuple(v.shape) or k.shape[0] != self.B \
-                or k.shape[1] != self.H or k.shape[3] != self.D:
+        if k.dim() != 4 or k.shape != v.shape or k.shape[0] != self.B or k.shape[1] != self.H \
+                or k.shape[3] != self.D:
             raise ValueError(f"KVCache8.append: k, v must be ({self.B},{self.H},T,{self.D})")
-        c, cp = (None, None) if counts is None else self._ints(counts, "counts")
-        with self._on(stream, k, v) as on:
-            check(_lib.load().gonn_hip_kvcache8_append(
-                self._live(), ctypes.byref(buf(k)), ctypes.byref(buf(v)), int(k.shape[2]), cp,
-                on.ptr), "KVCache8.append")
+        c = None if counts is None else self._ints(counts, "counts")
+        h, lib, kb, vb, T = self._live(), _lib.load(), buf(k), buf(v), k.shape[2]
+        self._run("KVCache8.append", lambda st: lib.gonn_hip_kvcache8_append(h, kb, vb, T, c, st),
+                  stream, k, v)
 
     def truncate(self, lengths, stream=None) -> None:
         """Drops the positions from lengths[b] on (host numbers). Any multiple of 64, or
         back to the start of the block before the one that the longest append so far
         ended in; the cache is then what it was at that length."""
-        n, p = self._ints(lengths, "lengths")
-        with self._on(stream) as on:
-            check(_lib.load().gonn_hip_kvcache8_truncate(self._live(), p, on.ptr),
-                  "KVCache8.truncate")
+        n, h, lib = self._ints(lengths, "lengths"), self._live(), _lib.load()
+        self._run("KVCache8.truncate", lambda st: lib.gonn_hip_kvcache8_truncate(h, n, st), stream)
 
     def reset(self, stream=None) -> None:
         """Drops every position."""
-        self.truncate(np.zeros(self.B), stream)
+        self.truncate((0,) * self.B, stream)
 
     def read(self, start=None, count=None, *, last=None, out=None, stream=None):
         """(k, v) bfloat16 (B,H,count,D): the numbers that positions start .. start +
@@ -830,15 +858,20 @@ class KVCache8:
             raise ValueError("KVCache8.read: give start and count, or last")
         n = int(last if last is not None else count)
         shape = (self.B, self.H, n, self.D)
-        with self._on(stream, *(out or ())) as on:
-            k, v = out if out is not None else (
-                torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        h, lib, first = self._live(), _lib.load(), -1 if last is not None else int(start)
+        if out is not None:
+            k, v = out
             for t in (k, v):
                 if tuple(t.shape) != shape:
                     raise ValueError(f"KVCache8.read: out must be {shape}")
-            check(_lib.load().gonn_hip_kvcache8_read(
-                self._live(), ctypes.byref(buf(k)), ctypes.byref(buf(v)),
-                -1 if last is not None else int(start), n, on.ptr), "KVCache8.read")
+        elif stream is None:
+            k, v = self._bf16.new_empty(shape), self._bf16.new_empty(shape)
+        else:
+            with self._on(stream):  # allocated where they are written
+                k, v = self._bf16.new_empty(shape), self._bf16.new_empty(shape)
+        kb, vb = buf(k), buf(v)
+        self._run("KVCache8.read", lambda st: lib.gonn_hip_kvcache8_read(h, kb, vb, first, n, st),
+                  stream, k, v)
         return k, v
 
     def attend(self, q, *, window: int = 0, sinks: int = 0, scale=None, out=None, stream=None):
@@ -854,19 +887,23 @@ class KVCache8:
         Hq, T = int(q.shape[1]), int(q.shape[2]) if q.dim() == 4 else 1
         if scale is None:
             scale = 1.0 / math.sqrt(self.D)
-        h, lib = self._live(), _lib.load()
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
+            raise ValueError("KVCache8.attend: out must be like q")
+        st = _plain_stream(self.device, stream, (q, out))
+        if st is not None:
+            return self._attend(q, Hq, T, window, sinks, scale, out, st, None)
         with self._on(stream, q, out) as on:
-            if out is None:
-                out = torch.empty_like(q)
-            elif tuple(out.shape) != tuple(q.shape) or out.dtype != q.dtype:
-                raise ValueError("KVCache8.attend: out must be like q")
-            need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, int(window), int(sinks),
-                                                                on.ptr)
-            ws = on.workspace(need)
-            check(lib.gonn_hip_kvcache8_attend(
-                h, ctypes.byref(buf(q)), ctypes.byref(buf(out)), Hq, T, float(scale), int(window),
-                int(sinks), ws.data_ptr() if ws is not None else None, need, on.ptr),
-                "KVCache8.attend")
+            return self._attend(q, Hq, T, window, sinks, scale, out, on.ptr, on._stream)
+
+    def _attend(self, q, Hq, T, window, sinks, scale, out, st, stream):
+        torch, h, lib = _torch(), self._live(), _lib.load()
+        if out is None:
+            out = torch.empty_like(q)
+        need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, int(window), int(sinks), st)
+        ws = _call_workspace(need, self.device, stream)
+        check(lib.gonn_hip_kvcache8_attend(
+            h, buf(q), buf(out), Hq, T, float(scale), int(window), int(sinks),
+            ws.data_ptr() if ws is not None else None, need, st), "KVCache8.attend")
         return out
 
 
