@@ -378,7 +378,8 @@ int check_window(const A* a, gonn::WindowParams* p) {
         return GONN_E_INVALID;
     if (a->window < 1 || a->sinks < 0 || !std::isfinite(a->scale)) return GONN_E_INVALID;
     if (!head_dim_ok(a->D)) return GONN_E_UNSUPPORTED;
-    // Grids and row numbers are 32-bit.
+    // Grids and row numbers are 32-bit, and so are the bf16 kernels' offsets in a head.
+    if ((double)std::max(a->Sq, a->Sk) * a->D * 2 >= 4.0e9) return GONN_E_UNSUPPORTED;
     if ((double)a->B * a->H * a->Sq >= 1073741824.0 || (double)a->B * a->Hkv * a->Sk >= 1073741824.0)
         return GONN_E_UNSUPPORTED;
     const int dt = a->q.dtype;

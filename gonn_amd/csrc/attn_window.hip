@@ -112,9 +112,18 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
     const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
     const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
 
+    constexpr bool DMA = NP == 1;
+    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
     Stage in;
-    in.init(tid);
-    if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    DmaStage<D, WK> dm;
+    const uint32_t lds = lds_addr(smem);
+    if constexpr (DMA) {
+        dm.init(tid);
+        if (nst > 0) dm.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
+    } else {
+        in.init(tid);
+        if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    }
     const T* qrow = (const T*)p.q + ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1)) * D;
     Frag<NP> qf[NKS];
     load_row_frags<D>(qrow, g, true, qf);
@@ -167,21 +176,31 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 oacc[t] = mfma_n(tile_col<D, NP>(tl, tile, 1, k, t), pf[k], oacc[t]);
     };
-    if (nst > 0) in.store(smem, tid);
-    __syncthreads();
-    for (int st = 0; st < nst; st++) {
-        const int buf = NBUF == 2 ? st & 1 : 0;
-        if (st + 1 < nst) in.load(Kg, Vg, ks.stage(st + 1) * BN, kl);
-        compute(st, buf);
-        if (NBUF == 1) __syncthreads();
-        if (st + 1 < nst) in.store(smem + (NBUF == 2 ? buf ^ 1 : 0) * STAGE, tid);
+    if constexpr (DMA) {
+        for (int st = 0; st < nst; st++) {
+            GONN_VMCNT(0);
+            __syncthreads();  // stage st has landed, and its buffer's last reader is past it
+            if (st + 1 < nst)
+                dm.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
+            compute(st, st & 1);
+        }
+    } else {
+        if (nst > 0) in.store(smem, tid);
         __syncthreads();
+        for (int st = 0; st < nst; st++) {
+            const int buf = NBUF == 2 ? st & 1 : 0;
+            if (st + 1 < nst) in.load(Kg, Vg, ks.stage(st + 1) * BN, kl);
+            compute(st, buf);
+            if (NBUF == 1) __syncthreads();
+            if (st + 1 < nst) in.store(smem + (NBUF == 2 ? buf ^ 1 : 0) * STAGE, tid);
+            __syncthreads();
+        }
     }
 
     // Key waves > 0 leave (o, m, l) in LDS, key wave 0 merges in order.
     auto merge = [&](float& l) {
         if constexpr (WK > 1) {
-            __syncthreads();
+            __syncthreads();  // every wave is past its last tile
             float* red = (float*)smem;
             if (wk > 0) {
                 float* d = red + ((wk - 1) * WQ + wq) * NE * 64 + lane;
@@ -543,9 +562,7 @@ void pick_window_fwd(const WindowParams& p, hipStream_t s) {
     const long long b128 = (long long)((p.Sq + 127) / 128) * BH;
     const long long b64 = (long long)((p.Sq + 63) / 64) * BH;
     if constexpr (sizeof(T) == 2) {
-        // The pipelined kernel reads a head's keys with 32-bit offsets.
-        const bool near = (double)p.Sk * D * 2 < 4.0e9;
-        if (b128 >= 2 * cus && near) window_fwd_pipe_kernel<D><<<(unsigned)b128, 256, 0, s>>>(p);
+        if (b128 >= 2 * cus) window_fwd_pipe_kernel<D><<<(unsigned)b128, 256, 0, s>>>(p);
         else if (b64 >= cus) run_window_fwd<D, T, 2, 2, 2>(p, s);
         else run_window_fwd<D, T, 1, 2, 1>(p, s);
     } else {

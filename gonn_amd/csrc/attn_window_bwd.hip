@@ -84,10 +84,12 @@ GONN_DEV void window_dq_plain(const WindowParams& p, int bh, int bk, int kl, con
 
 template <int D, typename T, int WB, int NBUF, int OCC>
 __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
-    constexpr int NS = 4 / WB, BM = WB * 32, BN = NS * 32, NP = kPlanes<T>;
+    constexpr int NP = kPlanes<T>, NS = 4 / WB, BM = WB * 32;
+    // Tiles of a stage per wave: two where four waves share a tile, which halves the barriers.
+    constexpr int KT = NP == 1 && NS == 1 ? 2 : 1, NT = NS * KT, BN = NT * 32;
     constexpr int NKS = D / 16, NDT = D / 32;
-    typedef RowStage<D, NS, T> Stage;
-    constexpr uint32_t STAGE = NS * Stage::TILE, RED = (NS - 1) * WB * NDT * 4096;
+    typedef RowStage<D, NT, T> Stage;
+    constexpr uint32_t STAGE = NT * Stage::TILE, RED = (NS - 1) * WB * NDT * 4096;
     __shared__ __attribute__((aligned(16))) char smem[NBUF * STAGE > RED ? NBUF * STAGE : RED];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -104,9 +106,18 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
     const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
     const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
 
+    constexpr bool DMA = NP == 1;
+    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
     Stage in;
-    in.init(tid);
-    if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    DmaStage<D, NT> dm;
+    const uint32_t lds = lds_addr(smem);
+    if constexpr (DMA) {
+        dm.init(tid);
+        if (nst > 0) dm.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
+    } else {
+        in.init(tid);
+        if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    }
     const size_t qr = ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1));
     const T* qrow = (const T*)p.q + qr * D;
     const T* grow = (const T*)p.dO + qr * D;
@@ -134,10 +145,10 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
     f32x16 acc[NDT];
     for (int t = 0; t < NDT; t++) acc[t] = f32x16{};
     const float c2 = p.scale_log2;
-    auto compute = [&](int st, int buf) {
-        const int kb = ks.stage(st) * BN + ws * 32;
+    auto compute = [&](int st, int buf, int x) {
+        const int kb = ks.stage(st) * BN + (ws * KT + x) * 32;
         if (kb >= kl || !band.any(qw, qw + 31, kb, kb + 31)) return;  // wave-uniform
-        char* tile = smem + buf * STAGE + ws * Stage::TILE;
+        char* tile = smem + buf * STAGE + (ws * KT + x) * Stage::TILE;
         f32x16 s = f32x16{}, dp = f32x16{};
         for (int k = 0; k < NKS; k++) {
             s = mfma_n(tile_row<D, NP>(tl, tile, 0, k), qf[k], s);
@@ -161,15 +172,26 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 acc[t] = mfma_n(tile_col<D, NP>(tl, tile, 0, k, t), df[k], acc[t]);
     };
-    if (nst > 0) in.store(smem, tid);
-    __syncthreads();
-    for (int st = 0; st < nst; st++) {
-        const int buf = NBUF == 2 ? st & 1 : 0;
-        if (st + 1 < nst) in.load(Kg, Vg, ks.stage(st + 1) * BN, kl);
-        compute(st, buf);
-        if (NBUF == 1) __syncthreads();
-        if (st + 1 < nst) in.store(smem + (NBUF == 2 ? buf ^ 1 : 0) * STAGE, tid);
+    if constexpr (DMA) {
+        for (int st = 0; st < nst; st++) {
+            GONN_VMCNT(0);
+            __syncthreads();  // stage st has landed, and its buffer's last reader is past it
+            if (st + 1 < nst)
+                dm.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
+            for (int x = 0; x < KT; x++) compute(st, st & 1, x);
+        }
+        if (NS > 1) __syncthreads();  // the merge reuses the stages
+    } else {
+        if (nst > 0) in.store(smem, tid);
         __syncthreads();
+        for (int st = 0; st < nst; st++) {
+            const int buf = NBUF == 2 ? st & 1 : 0;
+            if (st + 1 < nst) in.load(Kg, Vg, ks.stage(st + 1) * BN, kl);
+            compute(st, buf, 0);
+            if (NBUF == 1) __syncthreads();
+            if (st + 1 < nst) in.store(smem + (NBUF == 2 ? buf ^ 1 : 0) * STAGE, tid);
+            __syncthreads();
+        }
     }
     if (!merge_stream<NDT, WB, NS>(acc, smem, wb, ws, lane, NS)) return;
     {
@@ -342,13 +364,21 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     const int s1 = bs.nst * G - s0 > chunk ? s0 + chunk : bs.nst * G;
     if (it.part && s0 >= s1) return;  // no such item: nothing is read from its slot
 
+    constexpr bool DMA = NP == 1;
+    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
     Stage in;
-    in.init(tid);
+    DmaStage<D, NS> dm;
+    const uint32_t lds = lds_addr(smem);
+    if constexpr (DMA) dm.init(tid);
+    else in.init(tid);
     float rl = 0.f, rd = 0.f;
-    auto gload = [&](int st) {
+    // Step st: its rows (to buffer buf of LDS, or to registers), its L and D to registers.
+    auto gload = [&](int st, int buf) {
         const size_t bh = (size_t)b * p.H + hk * G + st / bs.nst;
         const int q0 = bs.q0 + st % bs.nst * BQ;
-        in.load((const T*)p.q + bh * p.Sq * D, (const T*)p.dO + bh * p.Sq * D, q0, p.Sq);
+        const T *Qg = (const T*)p.q + bh * p.Sq * D, *dOg = (const T*)p.dO + bh * p.Sq * D;
+        if constexpr (DMA) dm.load(Qg, dOg, q0, p.Sq, lds + buf * STAGE, wave);
+        else in.load(Qg, dOg, q0, p.Sq);
         if (tid < BQ) {
             const int q = q0 + tid;
             rl = q < p.Sp ? p.lse2[bh * p.Sp + q] : INFINITY;
@@ -356,13 +386,13 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
         }
     };
     auto sstore = [&](int buf) {
-        in.store(smem + buf * STAGE, tid);
+        if constexpr (!DMA) in.store(smem + buf * STAGE, tid);
         if (tid < BQ) {
             sld[buf][0][tid] = rl;
             sld[buf][1][tid] = rd;
         }
     };
-    if (s0 < s1) gload(s0);
+    if (s0 < s1) gload(s0, 0);
     const size_t kr = ((size_t)bk * p.Sk + (kj < p.Sk ? kj : p.Sk - 1)) * D;
     const T *krow = (const T*)p.k + kr, *vrow = (const T*)p.v + kr;
     Frag<NP> kf[NKS], vf[NKS];
@@ -412,15 +442,27 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 acc[NDT + t] = mfma_n(tile_col<D, NP>(tl, tile, 0, k, t), df[k], acc[NDT + t]);
     };
-    if (s0 < s1) sstore(0);
-    __syncthreads();
-    for (int st = s0; st < s1; st++) {
-        const int buf = NBUF == 2 ? (st - s0) & 1 : 0;
-        if (st + 1 < s1) gload(st + 1);
-        compute(st, buf);
-        if (NBUF == 1) __syncthreads();
-        if (st + 1 < s1) sstore(NBUF == 2 ? buf ^ 1 : 0);
+    if constexpr (DMA) {
+        for (int st = s0; st < s1; st++) {
+            const int buf = (st - s0) & 1;
+            sstore(buf);
+            GONN_VMCNT(0);
+            __syncthreads();  // step st has landed, and its buffer's last reader is past it
+            if (st + 1 < s1) gload(st + 1, buf ^ 1);
+            compute(st, buf);
+        }
+        if (NS > 1) __syncthreads();  // the merge reuses the stages
+    } else {
+        if (s0 < s1) sstore(0);
         __syncthreads();
+        for (int st = s0; st < s1; st++) {
+            const int buf = NBUF == 2 ? (st - s0) & 1 : 0;
+            if (st + 1 < s1) gload(st + 1, 0);
+            compute(st, buf);
+            if (NBUF == 1) __syncthreads();
+            if (st + 1 < s1) sstore(NBUF == 2 ? buf ^ 1 : 0);
+            __syncthreads();
+        }
     }
     if (!merge_stream<2 * NDT, WB, NS>(acc, smem, wb, ws, lane, NS)) return;
     {

@@ -171,7 +171,8 @@ typedef struct {
  * ptr NULL. Buffers 16-byte aligned. window >= 1 (Sq or more: no window),
  * sinks >= 0; kv_len: GONN_I32 device array [B] or ptr NULL, clamped to
  * [0, Sk]. An infinity or a NaN in a key or value reaches only the queries that
- * see that key.                                                            */
+ * see that key. GONN_E_UNSUPPORTED from B H Sq or B Hkv Sk = 2^30 on, and for
+ * heads of 2e9 elements or more (Sq D or Sk D).                            */
 typedef struct {
     gonn_buf q, k, v, o, lse;
     int B, H, Hkv, Sq, Sk, D;

@@ -78,3 +78,11 @@ def test_backward_needs_its_buffers_and_workspace():
     assert _lib.load().gonn_hip_attn_window_bwd(ctypes.byref(a), PTR, need - 1, None) == _lib.GONN_E_WORKSPACE
     assert _lib.load().gonn_hip_attn_workspace_bytes(
         _lib.GONN_OP_WINDOW_BWD, ctypes.byref(_args(_lib.WindowBwdArgs, window=0))) == 0
+
+
+@pytest.mark.parametrize("cls", [_lib.WindowFwdArgs, _lib.WindowBwdArgs])
+@pytest.mark.parametrize("dt", [_lib.GONN_BF16, _lib.GONN_F32])
+def test_heads_past_32_bit_offsets_are_refused(cls, dt):
+    one = dict(B=1, H=1, Hkv=1, D=128, window=64)
+    for kw in ({"Sq": 1 << 24}, {"Sk": 1 << 24}):
+        assert _call(_args(cls, dt, **one, **kw)) == _lib.GONN_E_UNSUPPORTED, kw
