@@ -2079,6 +2079,7 @@ int gonn_hip_kvcache8_free(gonn_kvcache8* h) {
 
 int gonn_hip_kvcache8_lengths(gonn_kvcache8* h, int* len, void* stream) {
     if (!h || !len) return GONN_E_INVALID;
+    if (h->captured && stream_captures((hipStream_t)stream)) return GONN_E_INVALID;  // would wait
     TRY(cache8_refresh(h, (hipStream_t)stream));
     std::copy(h->len.begin(), h->len.end(), len);
     return GONN_OK;
@@ -2092,13 +2093,15 @@ int gonn_hip_kvcache8_append(gonn_kvcache8* h, const gonn_buf* k, const gonn_buf
     const size_t n = (size_t)c.B * c.H * T * c.D;
     if (!buf_ok(*k, n, k->dtype) || !buf_ok(*v, n, v->dtype) || !aligned16(*k) || !aligned16(*v))
         return GONN_E_INVALID;
-    if ((double)c.B * c.H * ((double)T + 128) / 64 >= 2147483647.0) return GONN_E_UNSUPPORTED;
+    if (T > 1 << 30 || (double)c.B * c.H * ((double)T + 128) / 64 >= 2147483647.0)
+        return GONN_E_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     const bool capturing = stream_captures(s);
     if (!capturing) TRY(cache8_refresh(h, s));
     for (int b = 0; b < c.B; b++) {
         const int m = counts ? counts[b] : T;
-        if (m < 0 || m > T || (long long)h->len[b] + m > c.Lmax) return GONN_E_INVALID;
+        // The lengths that a captured append will meet are those of each replay.
+        if (m < 0 || m > T || (capturing ? 0LL : h->len[b]) + m > c.Lmax) return GONN_E_INVALID;
     }
     {
         ProfScope ps("kv8_append", s);
@@ -2176,8 +2179,9 @@ int gonn_hip_kvcache8_attend(gonn_kvcache8* h, const gonn_buf* q, gonn_buf* o, i
     a.o = o->ptr;
     a.Hq = Hq;
     a.T = T;
-    a.window = window;
-    a.sinks = window ? sinks : 0;
+    // Past Lmax every position is seen, and sums with positions stay in range.
+    a.window = std::min(window, h->c.Lmax);
+    a.sinks = window ? std::min(sinks, h->c.Lmax) : 0;
     a.rows = plan.rows;
     a.split = plan.split;
     a.nsplit = plan.nsplit;

@@ -166,7 +166,7 @@ struct RowStage {
 // The same tiles of bf16 tensors straight from memory to LDS (one plane each): nothing
 // passes through registers, so the load of the next stage needs none and its store none of
 // the wave's time. Complete behind GONN_VMCNT(0) and a barrier; one barrier a stage instead
-// of the two that a store from registers takes. dQ of 2 x 32 heads, 8192 queries, window
+// of the two that a store from registers takes. dQ of 2 x 16 heads, 8192 queries, window
 // 1024: 277 us through registers, 236 us this way. row0 < n, and n rows below 4 GB.
 template <int D, int NT>
 struct DmaStage {

@@ -698,10 +698,10 @@ __global__ __launch_bounds__(256, 2) void attend8_pipe_kernel(Attend8 a) {
     const brsrc krs = make_rsrc(c.k8 + bh * head, head), vrs = make_rsrc(c.v8 + bh * head, head);
     const uint32_t kvo = (uint32_t)((16 * wave + pr) * D + 16 * pc), vvo = (uint32_t)((16 * wave + pr) * kBlk8 + 16 * pc);
     auto load_k = [&](int t, int i) {
-        kst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, kvo + 64 * i, blk_of(t) * kBlk8 * D, 0));
+        kst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, kvo + 64 * i, (uint32_t)blk_of(t) * kBlk8 * D, 0));
     };
     auto load_v = [&](int t, int i) {
-        vst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, vvo + 64 * i * kBlk8, blk_of(t) * kBlk8 * D, 0));
+        vst[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, vvo + 64 * i * kBlk8, (uint32_t)blk_of(t) * kBlk8 * D, 0));
     };
     auto slot_pos = [&](int rows, int row, int chunk) {
         return (uint32_t)((((chunk >> 2) * rows + row) * 4 + ((chunk & 3) ^ slab_swz(row))) * 16);

@@ -489,6 +489,11 @@ def _call_workspace(nbytes, device, stream):
     return _WS.get(nbytes, device, stream)
 
 
+def _c_int(n):
+    """n as a C int, one that is out of range as the nearest limit (ctypes would wrap it)."""
+    return max(-0x80000000, min(int(n), 0x7fffffff))
+
+
 class _OnStream:
     """A call's device and stream, with the call's allocations on that stream;
     tensors used on a stream other than the current one are marked as used there,
@@ -584,7 +589,7 @@ def attn_window_fwd(q, k, v, *, window: int, sinks: int = 0, scale=None, kv_len=
         if lse_out is None and lse:
             lse_out = q.new_empty((B * H, Sq), dtype=torch.float32)
         a = WindowFwdArgs(buf(q), buf(k), buf(v), buf(out), buf(lse_out), B, H, Hkv, Sq, Sk, D,
-                          float(scale), int(window), int(sinks), buf(kv_len))
+                          float(scale), _c_int(window), _c_int(sinks), buf(kv_len))
         check(_lib.load().gonn_hip_attn_window_fwd(ctypes.byref(a), None, 0, on.ptr),
               "attn_window_fwd")
     return out, lse_out
@@ -611,7 +616,7 @@ def attn_window_bwd(q, k, v, o, lse, dO, *, window: int, sinks: int = 0, scale=N
             for name, t, ref in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
                 _window_like(what, name, t, ref)
         a = WindowBwdArgs(buf(q), buf(k), buf(v), buf(o), buf(lse), buf(dO), buf(dq), buf(dk),
-                          buf(dv), B, H, Hkv, Sq, Sk, D, float(scale), int(window), int(sinks),
+                          buf(dv), B, H, Hkv, Sq, Sk, D, float(scale), _c_int(window), _c_int(sinks),
                           buf(kv_len))
         lib = _lib.load()
         nb = lib.gonn_hip_attn_workspace_bytes(GONN_OP_WINDOW_BWD, ctypes.byref(a))
@@ -771,8 +776,8 @@ class KVCache8:
     def __init__(self, B: int, H: int, Lmax: int, D: int):
         self.B, self.H, self.Lmax, self.D = int(B), int(H), int(Lmax), int(D)
         self._h = ctypes.c_void_p()
-        check(_lib.load().gonn_hip_kvcache8_create(ctypes.byref(self._h), self.B, self.H,
-                                                   self.Lmax, self.D), "KVCache8")
+        check(_lib.load().gonn_hip_kvcache8_create(ctypes.byref(self._h),
+                                                   *map(_c_int, (B, H, Lmax, D))), "KVCache8")
         torch = _torch()
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._int_array = ctypes.c_int * self.B
@@ -811,6 +816,8 @@ class KVCache8:
             n = n.tolist()
         if len(n) != self.B:
             raise ValueError(f"KVCache8: {what} must have {self.B} entries")
+        if min(n) < -0x80000000 or max(n) > 0x7fffffff:
+            n = map(_c_int, n)
         return self._int_array(*n)
 
     def _run(self, what, call, stream, *tensors):
@@ -858,7 +865,7 @@ class KVCache8:
             raise ValueError("KVCache8.read: give start and count, or last")
         n = int(last if last is not None else count)
         shape = (self.B, self.H, n, self.D)
-        h, lib, first = self._live(), _lib.load(), -1 if last is not None else int(start)
+        h, lib, first = self._live(), _lib.load(), -1 if last is not None else _c_int(start)
         if out is not None:
             k, v = out
             for t in (k, v):
@@ -897,12 +904,13 @@ class KVCache8:
 
     def _attend(self, q, Hq, T, window, sinks, scale, out, st, stream):
         torch, h, lib = _torch(), self._live(), _lib.load()
+        window, sinks = _c_int(window), _c_int(sinks)
         if out is None:
             out = torch.empty_like(q)
-        need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, int(window), int(sinks), st)
+        need = lib.gonn_hip_kvcache8_attend_workspace_bytes(h, Hq, T, window, sinks, st)
         ws = _call_workspace(need, self.device, stream)
         check(lib.gonn_hip_kvcache8_attend(
-            h, buf(q), buf(out), Hq, T, float(scale), int(window), int(sinks),
+            h, buf(q), buf(out), Hq, T, float(scale), window, sinks,
             ws.data_ptr() if ws is not None else None, need, st), "KVCache8.attend")
         return out
 

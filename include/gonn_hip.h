@@ -255,8 +255,9 @@ int gonn_hip_attn_bwd(const gonn_attn_bwd_args* a, void* ws, size_t ws_bytes, vo
 
 /* Sliding-window attention with sinks, forward and backward (see the argument
  * structs). ws: gonn_hip_attn_workspace_bytes(GONN_OP_WINDOW_FWD / _BWD) bytes
- * (the forward needs none); calls that share one must not overlap. Only kernel
- * launches on `stream`: both can be captured in a HIP graph.               */
+ * (the forward needs none); calls that share one must not overlap. Outputs must
+ * not overlap inputs. Only kernel launches on `stream`: both can be captured in
+ * a HIP graph.                                                             */
 int gonn_hip_attn_window_fwd(const gonn_attn_window_fwd_args* a, void* ws, size_t ws_bytes,
                              void* stream);
 int gonn_hip_attn_window_bwd(const gonn_attn_window_bwd_args* a, void* ws, size_t ws_bytes,
@@ -350,10 +351,11 @@ int gonn_hip_kvcache_attend_causal(gonn_kvcache* c, const gonn_buf* q, gonn_buf*
  * All calls run on `stream` and none waits for it (except where noted); the
  * caller orders calls on different streams. Calls on one handle are not
  * reentrant. append, truncate, read and attend can be captured in a HIP graph
- * (lengths live on the device; a replayed append that would pass Lmax leaves that
- * sequence as it is). After a captured append or truncate the host no longer
- * knows the lengths: lengths, truncate and append then read them back first,
- * which waits for `stream`.                                                */
+ * (lengths live on the device: a replay works on those it meets, and an append that
+ * would pass Lmax leaves that sequence as it is). Outputs must not overlap inputs.
+ * After a captured append or truncate the host no longer knows the lengths: lengths,
+ * truncate and append then read them back first, which waits for `stream` (and
+ * lengths, which cannot wait in a capture, returns GONN_E_INVALID in one).  */
 typedef struct gonn_kvcache8 gonn_kvcache8;
 
 /* D must be 64 or 128 (GONN_E_UNSUPPORTED otherwise). *out is NULL on failure. */
@@ -562,10 +564,11 @@ double gonn_hip_bench_flash_attn_f64_bwd(int BH, int S, int d, int iters, int ca
 /* Per-kernel event profiler. While enabled, every kernel stage this library
  * launches ("pack_kv", "fwd_bf16", "fwd_f32", "decode_split",
  * "decode_combine", "decode_causal_split", "decode_causal_combine", "bwd_prep",
- * "bwd_pack", "bwd_dkdv", "bwd_dq") is bracketed by two HIP events on its own
- * stream. profile_read synchronises on the recorded events
- * and returns the summed milliseconds and launch count of one stage. No
- * reference counterpart: the reference times whole launches with CUDA events
+ * "bwd_pack", "bwd_dkdv", "bwd_dq", "window_fwd", "window_bwd", "kv8_append",
+ * "kv8_attend") is bracketed by two HIP events on its own
+ * stream. profile_read synchronises on the recorded events and returns the summed
+ * milliseconds and launch count of one stage. No reference counterpart: the
+ * reference times whole launches with CUDA events
  * (backend/cuda/gonn_cuda.cu:548-559).                                    */
 int gonn_hip_profile_enable(int on);
 int gonn_hip_profile_reset(void);

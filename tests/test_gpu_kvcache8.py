@@ -313,3 +313,94 @@ def test_refusals():
         c.attend(q)
     with pytest.raises(ValueError):
         c.lengths()
+
+
+@pytest.mark.parametrize("T", [1, 30, 90, 150])
+def test_widest_window_with_rows_ahead_of_the_sequence(T):
+    """Queries at positions below zero see nothing, whatever the window, and a window or a
+    number of sinks past 32 bits is the widest one."""
+    from gonn_amd import hip
+    B, Hq, H, D, lens = 2, 2, 1, 64, [40, 20]
+    k, v = (_rows(B, H, 64, D, 110 + i) for i in range(2))
+    q = _rows(B, Hq, T, D, 112)
+    with hip.KVCache8(B, H, 64, D) as c:
+        c.append(k.cuda(), v.cuda(), counts=lens)
+        want = c.attend(q.cuda())
+        for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 40, 2 ** 40), (1, 2 ** 40)):
+            assert torch.equal(c.attend(q.cuda(), window=window, sinks=sinks), want), (window, sinks)
+        for b, n in enumerate(lens):
+            assert not want[b, :, :max(T - n, 0)].any()
+            assert want[b, :, max(T - n, 0):].any()
+
+
+def test_numbers_past_32_bits_are_refused():
+    from gonn_amd import hip
+    k = _rows(2, 1, 10, 64, 113).cuda()
+    with hip.KVCache8(2, 1, 64, 64) as c:
+        for call in (lambda: c.append(k, k, counts=[2 ** 32 + 1, 1]), lambda: c.truncate([-2 ** 32, 0]),
+                     lambda: c.read(2 ** 32, 1), lambda: hip.KVCache8(1, 1, 2 ** 32 + 64, 64)):
+            with pytest.raises(hip.GonnHipError):
+                call()
+        assert list(c.lengths()) == [0, 0]
+
+
+def test_captured_refill_of_a_full_cache():
+    """What the host knows of the lengths when a graph is captured is not what its replays meet."""
+    from gonn_amd import hip
+    B, H, D, Lmax = 2, 2, 64, 130
+    k, v = (_rows(B, H, Lmax, D, 115 + i).cuda() for i in range(2))
+    with hip.KVCache8(B, H, Lmax, D) as c:
+        c.append(k, v)
+        c.reset()
+        c.append(v, k)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.reset()
+            c.append(k, v)
+            with pytest.raises(hip.GonnHipError):
+                c.append(torch.cat([k, k], 2), torch.cat([k, k], 2))  # never fits
+            with pytest.raises(hip.GonnHipError):
+                c.lengths()  # would wait
+            got = c.read(0, Lmax)
+        for t in range(3):
+            k.copy_(torch.roll(k, 1, 2))
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert list(c.lengths()) == [Lmax] * B
+            for b in range(B):
+                assert _same(got[0][b], ref.held(k[b].cpu(), Lmax)) and _same(got[1][b], ref.held(v[b].cpu(), Lmax))
+            c.truncate([64, 0])
+
+
+def test_offsets_past_32_bits():
+    """A head of more than 4e9 codes: every kernel finds the first positions and the last."""
+    from gonn_amd import hip
+    D, step, n = 128, 1 << 20, (1 << 25) + (1 << 20) - 40
+    g = torch.Generator(device="cuda").manual_seed(7)
+    rows = torch.randn(1, 1, step, D, generator=g, device="cuda").bfloat16()
+    with hip.KVCache8(1, 1, n, D) as c:
+        for a in range(0, n, step):
+            # The rows of a block of positions, told apart from the others' by their sign and order.
+            x = torch.roll(rows, a // step * 97, 2)
+            m = min(step, n - a)
+            c.append(x[:, :, :m].contiguous(), -x[:, :, :m].contiguous())
+        assert list(c.lengths()) == [n]
+        a = (n - 1) // step * step
+        x = torch.roll(rows, a // step * 97, 2)[:, :, n - a - 200:n - a]
+        tail = c.read(last=200)
+        lead = (n - 200) % 64  # whole blocks from here on, the open one last
+        want = ref.held(x[0].cpu()[:, 64 - lead:], 200 - (64 - lead))
+        assert _same(tail[0][0, :, 64 - lead:], want) and _same(tail[1][0, :, 64 - lead:], -want)
+        head = c.read(0, 128)
+        assert _same(head[0][0], ref.held(rows[0, :, :128].cpu(), 128))
+        # Window and sinks: positions of both ends, in each form of the attention.
+        held_k = torch.cat([head[0], c.read(last=512)[0]], 2)[0].cpu().double()
+        held_v = torch.cat([head[1], c.read(last=512)[1]], 2)[0].cpu().double()
+        for T, dtype in ((1, torch.bfloat16), (1, torch.float32), (30, torch.bfloat16), (60, torch.float32),
+                         (130, torch.bfloat16), (130, torch.float32)):
+            q = _rows(1, 1, T, D, 120, dtype)
+            o = c.attend(q.cuda(), window=300, sinks=128).cpu()
+            ro, ra = ref.attend(q[0], held_k, held_v, 1 / math.sqrt(D), 300, 128)
+            check(o[0], ro, ra, f"{T} queries {dtype}")
