@@ -869,6 +869,11 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     const long long want = (p.rows == 128 ? 2 : 4) * cus;
     const long long least = p.rows <= 32 ? (blocks <= 24 ? blocks : 8) : 128 / p.rows;
     long long split = 64;
+    // Many rows are bound by their products, and each split costs a row 4 D bytes more of
+    // partials: no more splits than four workgroups per CU (8 key heads of 32768 positions,
+    // 4 x 2048 rows each, D 128: 8 splits 1067 us, 2 1007; 65536 positions and 8 x 4096
+    // rows: 16 splits 8.5 ms and 2.1 GB of partials, one 7.7).
+    if (p.rows == 128) split = std::max(split, blocks * units / (4 * cus));
     if (units * ((blocks + split - 1) / split) < want)
         split = std::min(split, std::max(least, blocks * units / want));
     p.split = (int)std::max<long long>(1, split);
