@@ -266,3 +266,42 @@ def test_refusals():
         hip.attn_window_bwd(q, k, v, o.float(), lse, dO, window=4)
     with pytest.raises(hip.GonnHipError):
         hip.attn_window_bwd(q, k, v, o, lse[:2].contiguous(), dO, window=4)
+
+
+def test_windows_past_32_bits_are_the_widest():
+    from gonn_amd import hip
+    q, k, v, dO = _data((1, 2, 1, 90, 90, 64), torch.bfloat16, 31)
+    o, lse = hip.attn_window_fwd(q, k, v, window=90)
+    want = hip.attn_window_bwd(q, k, v, o, lse, dO, window=90)
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 32 + 5, 2 ** 32 + 1), (2 ** 63, 2 ** 31 - 1)):
+        o2, lse2 = hip.attn_window_fwd(q, k, v, window=window, sinks=sinks)
+        assert torch.equal(o2, o) and torch.equal(lse2, lse)
+        got = hip.attn_window_bwd(q, k, v, o, lse, dO, window=window, sinks=sinks)
+        for a, b in zip(got, want):  # other items, another order of the sums
+            assert ((a.double() - b.double()).abs() <= 2.0 ** -6 * b.double().abs() + 2.0 ** -8).all()
+    with pytest.raises(hip.GonnHipError):
+        hip.attn_window_fwd(q, k, v, window=2 ** 32 + 5, sinks=-2 ** 32)
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^32 elements: the last head's last rows, which see the last keys
+    and the sinks. The reference is the same attention with the rows between left out; it
+    holds for the queries whose windows end within what is kept."""
+    from gonn_amd import hip
+    B, H, S, D, window, sinks, keep, n = 8, 8, 524_353, 128, 100, 3, 512, 256
+    assert B * H * S * D > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(3)
+    mk = lambda: torch.randn(B, H, S, D, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    q, k, v, dO = (mk() for _ in range(4))
+    o, lse = hip.attn_window_fwd(q, k, v, window=window, sinks=sinks)
+    grads = hip.attn_window_bwd(q, k, v, o, lse, dO, window=window, sinks=sinks)
+    part = lambda x: torch.cat([x[-1:, -1:, :64], x[-1:, -1:, S - keep:]], 2).cpu()  # noqa: E731
+    last = lambda x: x[..., -n:, :]  # noqa: E731
+    scale = 1.0 / math.sqrt(D)
+    ro, rl, ra = ref.fwd(part(q), part(k), part(v), scale, window, sinks)
+    ref.check(last(part(o)), last(ro), last(ra), "o")
+    le = part(lse.view(B, H, S, 1))[..., 0]
+    _check_lse(le[..., -n:], rl[..., -n:], "lse")
+    rg, rs, rn = ref.bwd(part(q), part(k), part(v), part(o), le, part(dO), scale, window, sinks)
+    for name, x, r, s, m in zip(("dq", "dk", "dv"), grads, rg, rs, rn):
+        ref.check(last(part(x)), last(r), last(s), name, last(m))
