@@ -848,34 +848,44 @@ Plan8 attend8_plan(const gonn_kvcache8* h, int Hq, int T, int window, int sinks,
     const long long R = (long long)Hq / c.H * T, cus = gonn::device_cus();
     Plan8 p{};
     p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
-    int longest = c.Lmax;
-    if (!h->captured && !stream_captures(s)) longest = *std::max_element(h->len.begin(), h->len.end());
-    long long blocks = (longest + gonn::kBlk8 - 1) / gonn::kBlk8;
-    if (window > 0) {
-        const long long seen = ((long long)window + T + 2 * gonn::kBlk8 - 3) / gonn::kBlk8 +
-                               ((long long)sinks + gonn::kBlk8 - 1) / gonn::kBlk8;
-        blocks = std::min(blocks, seen);
-    }
-    blocks = std::max<long long>(blocks, 1);
-    const long long units = (long long)c.B * c.H * ((R + p.rows - 1) / p.rows);
-    // Splits of 64 blocks: a workgroup's start and merge cost its CU about 2 us, so
-    // long ones stream faster (2048 heads of 8192 positions, D 128: 16 blocks 5.4
-    // TB/s, 32 6.2, 64 6.6, 128 6.9), but sequences of different lengths level out
-    // less (512 to 8192: 441, 397, 387, 390 us). Shorter ones where the device has
-    // room for more workgroups, down to two blocks per key wave; but no more than one
-    // split for up to 24 blocks, which spares the second kernel (8 heads, D 128, 16
-    // blocks 11 us against 16, replayed 11 against 12; 32 blocks 16 and 16, replayed
-    // 16 and 12; 64 blocks in splits of 4, 8 and 16: 16, 14, 15 us replayed).
-    const long long want = (p.rows == 128 ? 2 : 4) * cus;
+    // Blocks that the longest sequence's rows and all the sequences' see.
+    const bool known = !h->captured && !stream_captures(s);
+    const long long seen = window > 0 ? ((long long)window + T + 2 * gonn::kBlk8 - 3) / gonn::kBlk8 +
+                                            ((long long)sinks + gonn::kBlk8 - 1) / gonn::kBlk8
+                                      : (long long)c.Lmax;
+    auto sees = [&](int b) {
+        const long long l = known ? h->len[b] : c.Lmax;
+        return std::min((l + gonn::kBlk8 - 1) / gonn::kBlk8, seen);
+    };
+    const long long units = c.H * ((R + p.rows - 1) / p.rows);  // of a sequence
+    auto workgroups = [&](long long split) {
+        long long n = 0;
+        for (int b = 0; b < c.B; b++) n += (sees(b) + split - 1) / split;
+        return n * units;
+    };
+    long long blocks = 1;
+    for (int b = 0; b < c.B; b++) blocks = std::max(blocks, sees(b));
+    const long long total = workgroups(1);
+    // Four workgroups per CU, the longest first (turn_of in kvcache8_attend.hip), and no
+    // more: a workgroup's start and merge cost its CU about 2 us, so long splits stream
+    // faster (2048 heads of 8192 positions, D 128, one row: 16 blocks 5.4 TB/s, 32 6.0, 64
+    // 6.3, 128 6.7; of 512 to 8192 positions: 414 us in splits of 32, 390 of 64, 356 of
+    // 128), and each split costs a row 4 D bytes of partials (8 key heads of 32768
+    // positions, 4 x 2048 rows each, D 128: 8 splits 1067 us, 2 1007). Not fewer than 8
+    // blocks in a split of one matrix tile's rows, two per key wave, and no more than one
+    // such split for up to 24 blocks, which spares the second kernel (8 heads, D 128, 16
+    // blocks 11 us against 16, replayed 11 against 12; 32 blocks 16 and 16, replayed 16
+    // and 12; 64 blocks in splits of 4, 8 and 16: 16, 14, 15 us replayed). 128 rows:
+    // two workgroups per CU in one round, where that leaves less than 64 blocks to each
+    // (8 x 4 sequences of 2048 to 4096, 4 x 256 rows: 77 us; a few more workgroups 81).
     const long long least = p.rows <= 32 ? (blocks <= 24 ? blocks : 8) : 128 / p.rows;
-    long long split = 64;
-    // Many rows are bound by their products, and each split costs a row 4 D bytes more of
-    // partials: no more splits than four workgroups per CU (8 key heads of 32768 positions,
-    // 4 x 2048 rows each, D 128: 8 splits 1067 us, 2 1007; 65536 positions and 8 x 4096
-    // rows: 16 splits 8.5 ms and 2.1 GB of partials, one 7.7).
-    if (p.rows == 128) split = std::max(split, blocks * units / (4 * cus));
-    if (units * ((blocks + split - 1) / split) < want)
-        split = std::min(split, std::max(least, blocks * units / want));
+    long long split = total / (4 * cus);
+    if (split < 64) {
+        split = std::max(least, p.rows == 128 ? total / (2 * cus) : split);
+        if (p.rows == 128)
+            while (split < 64 && workgroups(split) > 2 * cus) split++;
+        split = std::min(split, 64LL);
+    }
     p.split = (int)std::max<long long>(1, split);
     p.nsplit = (int)((blocks + p.split - 1) / p.split);
     return p;

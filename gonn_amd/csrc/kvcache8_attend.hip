@@ -74,6 +74,38 @@ GONN_DEV int splits8(const Attend8& a, int nv) {
     return ns < a.nsplit ? ns : a.nsplit;
 }
 
+// Split and head of the workgroup whose turn is `us`, for rows of queries t0 ..
+// t1: of every 64 sequences those with the longest splits first. A workgroup streams 64
+// blocks for about 80 us, and one that starts last leaves the device idle for as long.
+// With the later splits, which only long sequences have, ahead of the first ones, short
+// sequences are left for the end. (2048 heads, 512 to 8192 positions, D 128, one row: 390
+// us in the order of the sequences, in splits of 64 blocks; 356 this way, in splits of 128.)
+struct Turn8 {
+    int sp, len;  // split; the sequence's length
+    size_t bh;    // its row of heads
+};
+GONN_DEV Turn8 turn_of(const Attend8& a, int us, int t0, int t1, int lane) {
+    const Cache8& c = a.c;
+    const int BH = c.B * c.H, order = us / BH, at = us - order * BH, place = at / c.H;
+    const int g0 = place & ~63, nb = c.B - g0 < 64 ? c.B - g0 : 64;
+    int key = -1, len = 0;
+    if (lane < nb) {
+        len = c.len[g0 + lane];
+        len = len < c.Lmax ? len : c.Lmax;
+        Blocks8 bs;
+        bs.init(len - a.T + t0, len - a.T + t1, a.window, a.sinks);
+        const int nv = bs.count(), ns = splits8(a, nv);
+        key = (ns ? (nv + ns - 1) / ns : 0) * 64 + 63 - lane;  // all different; under 2^31
+    }
+    int before = 0;
+    for (int j = 0; j < nb; j++) before += __builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < nb && before == (place & 63));
+    const int at_lane = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+    return {__builtin_amdgcn_readfirstlane(a.nsplit - 1 - order),
+            __builtin_amdgcn_readlane(len, at_lane),
+            (size_t)(g0 + at_lane) * c.H + __builtin_amdgcn_readfirstlane(at - place * c.H)};
+}
+
 GONN_DEV bool sees8(int i, int j, int window, int sinks) {
     return j <= i && (window == 0 || i - j < window || j < sinks);
 }
@@ -226,16 +258,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attend8_kernel(At
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wq = wave % WQ, wk = wave / WQ, g = lane >> 5, ln = lane & 31;
     const int T_ = a.T, R = a.Hq / c.H * T_, nrb = (R + BM - 1) / BM, BH = c.B * c.H;
-    // All first splits before the second ones, which short sequences do not have.
     int us, rb;
     map_block(blockIdx.x, nrb, BH * a.nsplit, true, us, rb, 1, true);
-    const int sp = __builtin_amdgcn_readfirstlane(us / BH), bhi = us - sp * BH, b = bhi / c.H;
-    const size_t bh = bhi;
-    int len = c.len[b];
-    len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
     const int r0 = rb * BM, r1 = r0 + BM < R ? r0 + BM : R;
     int t0, t1;
     query_span(r0, r1 - 1, T_, t0, t1);
+    const Turn8 turn = turn_of(a, us, t0, t1, lane);
+    const int sp = turn.sp, len = turn.len;
+    const size_t bh = turn.bh;
     Blocks8 bs;
     bs.init(len - T_ + t0, len - T_ + t1, a.window, a.sinks);
     const int nv = bs.count(), ns = splits8(a, nv);
@@ -453,14 +483,11 @@ __global__ __launch_bounds__(256, 2) void attend8_few_kernel(Attend8 a) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int wk = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
     const int T_ = a.T, R = a.Hq / c.H * T_, BH = c.B * c.H;
-    int us, rb;
-    map_block(blockIdx.x, 1, BH * a.nsplit, false, us, rb, 1, true);
-    const int sp = __builtin_amdgcn_readfirstlane(us / BH), bhi = us - sp * BH, b = bhi / c.H;
-    const size_t bh = bhi;
-    int len = c.len[b];
-    len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
     int t0, t1;
     query_span(0, R - 1, T_, t0, t1);
+    const Turn8 turn = turn_of(a, blockIdx.x, t0, t1, lane);
+    const int sp = turn.sp, len = turn.len;
+    const size_t bh = turn.bh;
     Blocks8 bs;
     bs.init(len - T_ + t0, len - T_ + t1, a.window, a.sinks);
     const int nv = bs.count(), ns = splits8(a, nv);
@@ -655,13 +682,12 @@ __global__ __launch_bounds__(256, 2) void attend8_pipe_kernel(Attend8 a) {
     const int T_ = a.T, R = a.Hq / c.H * T_, nrb = (R + BM - 1) / BM, BH = c.B * c.H;
     int us, rb;
     map_block(blockIdx.x, nrb, BH * a.nsplit, true, us, rb, 1, true);
-    const int sp = __builtin_amdgcn_readfirstlane(us / BH), bhi = us - sp * BH, b = bhi / c.H;
-    const size_t bh = bhi;
-    int len = c.len[b];
-    len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
     const int r0 = rb * BM, r1 = r0 + BM < R ? r0 + BM : R;
     int t0, t1;
     query_span(r0, r1 - 1, T_, t0, t1);
+    const Turn8 turn = turn_of(a, us, t0, t1, lane);
+    const int sp = turn.sp, len = turn.len;
+    const size_t bh = turn.bh;
     Blocks8 bs;
     bs.init(len - T_ + t0, len - T_ + t1, a.window, a.sinks);
     const int nv = bs.count(), ns = splits8(a, nv);

@@ -404,3 +404,33 @@ def test_offsets_past_32_bits():
             o = c.attend(q.cuda(), window=300, sinks=128).cpu()
             ro, ra = ref.attend(q[0], held_k, held_v, 1 / math.sqrt(D), 300, 128)
             check(o[0], ro, ra, f"{T} queries {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T", [1, 20, 50, 130])
+def test_many_sequences_of_different_lengths(T, dtype):
+    """More sequences than lanes, of one split to several, empty ones among them: each has its
+    turn, in a call that knows the lengths and in a captured one."""
+    from gonn_amd import hip
+    B, Hq, H, D, Lmax = 70, 2, 1, 64, 1700
+    lens = [(i * 577) % (Lmax + 1) if i % 9 else 0 for i in range(B)]
+    lens[5] = Lmax
+    k, v = (_rows(B, H, Lmax, D, 130 + i) for i in range(2))
+    q = _rows(B, Hq, T, D, 132, dtype)
+    with hip.KVCache8(B, H, Lmax, D) as c:
+        c.append(k.cuda(), v.cuda(), counts=lens)
+        qd = q.cuda()
+        o = c.attend(qd, window=900, sinks=70)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            og = c.attend(qd, window=900, sinks=70)
+        for _ in range(2):
+            og.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+    some = list(range(0, B, 4)) + [5, 63, 65, 69]
+    ro, ra = zip(*(ref.attend(q[b], ref.held(k[b], lens[b]), ref.held(v[b], lens[b]), 1 / math.sqrt(D), 900, 70)
+                   for b in some))
+    for got in (o, og):
+        check(torch.stack([got[b].cpu() for b in some]), torch.stack(ro), torch.stack(ra), f"{T} queries")
