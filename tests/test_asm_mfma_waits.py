@@ -1,11 +1,10 @@
 """Wait states between MFMAs and the first use of their results, over every path (CPU).
 
 A VALU or memory instruction may read or overwrite an MFMA's result only some wait states
-after it: 7 for v_mfma_f32_16x16x32_bf16, 11 for
-32x32x16, 18 for v_mfma_f32_32x32x2_f32 (an MFMA that
-accumulates onto it needs none). The compiler inserts them, but where it sank the reading
-instructions below a branch it has inserted too few on the taken path, and the last
-registers of a result were read before they were written. pin_before_branch (common.h)
+after it: 7 for v_mfma_f32_16x16x32_bf16, 11 for 32x32x16, 18 for v_mfma_f32_32x32x2_f32
+(an MFMA that accumulates onto it needs none). The compiler inserts them, but where it sank
+the reading instructions below a branch it has inserted too few on the taken path, and the
+last registers of a result were read before they were written. pin_before_branch (common.h)
 prevents that in the sources; this test compiles the window and 8-bit cache kernels with
 the build's flags and follows every path behind every MFMA.
 """
