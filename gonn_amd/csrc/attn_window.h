@@ -122,12 +122,17 @@ GONN_DEV void store4(T* p, f32x4 v) {
     }
 }
 
-// The streamed side of a stage: NT tiles of 32 rows of two tensors, loaded one
-// stage ahead into registers and stored as operand planes (SplitTile's layout:
-// the first tensor's planes, then the second's). Rows at and past n are zeros.
+// The streamed side of a stage: NT tiles of 32 rows of two tensors, in LDS as operand
+// planes (SplitTile's layout: the first tensor's planes, then the second's). Rows at and
+// past n are zeros.
 template <int D, int NT, typename T>
-struct RowStage {
-    static constexpr int NP = kPlanes<T>, NCH = 32 * D / 8, CH = NT * NCH / 256;
+struct RowStage;
+// fp32: loaded one stage ahead into registers, split and stored.
+template <int D, int NT>
+struct RowStage<D, NT, float> {
+    typedef float T;
+    static constexpr bool DIRECT = false;
+    static constexpr int NP = 3, NCH = 32 * D / 8, CH = NT * NCH / 256;
     static constexpr uint32_t PB = 32 * D * 2, TILE = 2 * NP * PB;
     Raw8<T> r[CH][2];
     int row[CH], col[CH];
@@ -163,13 +168,13 @@ struct RowStage {
         }
     }
 };
-// The same tiles of bf16 tensors straight from memory to LDS (one plane each): nothing
-// passes through registers, so the load of the next stage needs none and its store none of
-// the wave's time. Complete behind GONN_VMCNT(0) and a barrier; one barrier a stage instead
+// bf16: straight from memory to LDS (one plane each), so that the load of the next stage
+// needs no registers and its store none of the wave's time. Complete behind GONN_VMCNT(0) and a barrier; one barrier a stage instead
 // of the two that a store from registers takes. dQ of 2 x 16 heads, 8192 queries, window
 // 1024: 277 us through registers, 236 us this way. row0 < n, and n rows below 4 GB.
 template <int D, int NT>
-struct DmaStage {
+struct RowStage<D, NT, bf16> {
+    static constexpr bool DIRECT = true;
     static constexpr int NCH = 32 * D / 8, CH = NT * NCH / 256;
     static constexpr uint32_t PB = 32 * D * 2, TILE = 2 * PB;
     uint32_t off[CH];

@@ -124,17 +124,13 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
     const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
     const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
 
-    constexpr bool DMA = NP == 1;
-    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
-    Stage in;
-    DmaStage<D, WK> dm;
+    static_assert(!Stage::DIRECT || NBUF == 2, "loads to LDS need the other buffer");
     const uint32_t lds = lds_addr(smem);
-    if constexpr (DMA) {
-        dm.init(tid);
-        if (nst > 0) dm.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
-    } else {
-        in.init(tid);
-        if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    Stage in;
+    in.init(tid);
+    if (nst > 0) {
+        if constexpr (Stage::DIRECT) in.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
+        else in.load(Kg, Vg, ks.stage(0) * BN, kl);
     }
     const T* qrow = (const T*)p.q + ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1)) * D;
     Frag<NP> qf[NKS];
@@ -188,12 +184,12 @@ __global__ __launch_bounds__(256, OCC) void window_fwd_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 oacc[t] = mfma_n(tile_col<D, NP>(tl, tile, 1, k, t), pf[k], oacc[t]);
     };
-    if constexpr (DMA) {
+    if constexpr (Stage::DIRECT) {
         for (int st = 0; st < nst; st++) {
             GONN_VMCNT(0);
             __syncthreads();  // stage st has landed, and its buffer's last reader is past it
             if (st + 1 < nst)
-                dm.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
+                in.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
             compute(st, st & 1);
         }
     } else {

@@ -118,17 +118,13 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
     const T* Kg = (const T*)p.k + (size_t)bk * p.Sk * D;
     const T* Vg = (const T*)p.v + (size_t)bk * p.Sk * D;
 
-    constexpr bool DMA = NP == 1;
-    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
-    Stage in;
-    DmaStage<D, NT> dm;
+    static_assert(!Stage::DIRECT || NBUF == 2, "loads to LDS need the other buffer");
     const uint32_t lds = lds_addr(smem);
-    if constexpr (DMA) {
-        dm.init(tid);
-        if (nst > 0) dm.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
-    } else {
-        in.init(tid);
-        if (nst > 0) in.load(Kg, Vg, ks.stage(0) * BN, kl);
+    Stage in;
+    in.init(tid);
+    if (nst > 0) {
+        if constexpr (Stage::DIRECT) in.load(Kg, Vg, ks.stage(0) * BN, kl, lds, wave);
+        else in.load(Kg, Vg, ks.stage(0) * BN, kl);
     }
     const size_t qr = ((size_t)bh * p.Sq + (qi < p.Sq ? qi : p.Sq - 1));
     const T* qrow = (const T*)p.q + qr * D;
@@ -184,12 +180,12 @@ __global__ __launch_bounds__(256, OCC) void window_dq_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 acc[t] = mfma_n(tile_col<D, NP>(tl, tile, 0, k, t), df[k], acc[t]);
     };
-    if constexpr (DMA) {
+    if constexpr (Stage::DIRECT) {
         for (int st = 0; st < nst; st++) {
             GONN_VMCNT(0);
             __syncthreads();  // stage st has landed, and its buffer's last reader is past it
             if (st + 1 < nst)
-                dm.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
+                in.load(Kg, Vg, ks.stage(st + 1) * BN, kl, lds + (uint32_t)((st + 1) & 1) * STAGE, wave);
             for (int x = 0; x < KT; x++) compute(st, st & 1, x);
         }
         if (NS > 1) __syncthreads();  // the merge reuses the stages
@@ -376,20 +372,17 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
     const int s1 = bs.nst * G - s0 > chunk ? s0 + chunk : bs.nst * G;
     if (it.part && s0 >= s1) return;  // no such item: nothing is read from its slot
 
-    constexpr bool DMA = NP == 1;
-    static_assert(!DMA || NBUF == 2, "loads to LDS need the other buffer");
-    Stage in;
-    DmaStage<D, NS> dm;
+    static_assert(!Stage::DIRECT || NBUF == 2, "loads to LDS need the other buffer");
     const uint32_t lds = lds_addr(smem);
-    if constexpr (DMA) dm.init(tid);
-    else in.init(tid);
+    Stage in;
+    in.init(tid);
     float rl = 0.f, rd = 0.f;
     // Step st: its rows (to buffer buf of LDS, or to registers), its L and D to registers.
     auto gload = [&](int st, int buf) {
         const size_t bh = (size_t)b * p.H + hk * G + st / bs.nst;
         const int q0 = bs.q0 + st % bs.nst * BQ;
         const T *Qg = (const T*)p.q + bh * p.Sq * D, *dOg = (const T*)p.dO + bh * p.Sq * D;
-        if constexpr (DMA) dm.load(Qg, dOg, q0, p.Sq, lds + buf * STAGE, wave);
+        if constexpr (Stage::DIRECT) in.load(Qg, dOg, q0, p.Sq, lds + buf * STAGE, wave);
         else in.load(Qg, dOg, q0, p.Sq);
         if (tid < BQ) {
             const int q = q0 + tid;
@@ -398,7 +391,7 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
         }
     };
     auto sstore = [&](int buf) {
-        if constexpr (!DMA) in.store(smem + buf * STAGE, tid);
+        if constexpr (!Stage::DIRECT) in.store(smem + buf * STAGE, tid);
         if (tid < BQ) {
             sld[buf][0][tid] = rl;
             sld[buf][1][tid] = rd;
@@ -454,7 +447,7 @@ __global__ __launch_bounds__(256, OCC) void window_dkdv_kernel(WindowParams p) {
             for (int t = 0; t < NDT; t++)
                 acc[NDT + t] = mfma_n(tile_col<D, NP>(tl, tile, 0, k, t), df[k], acc[NDT + t]);
     };
-    if constexpr (DMA) {
+    if constexpr (Stage::DIRECT) {
         for (int st = s0; st < s1; st++) {
             const int buf = (st - s0) & 1;
             sstore(buf);
