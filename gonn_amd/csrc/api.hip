@@ -798,8 +798,8 @@ struct gonn_kvcache8 {
     gonn::Cache8 c{};
     void* mem = nullptr;  // everything on the device
     std::vector<int> len, lo;
-    // A call that changes the lengths was captured in a graph: they may advance
-    // without the host, which reads them back where it needs them.
+    // A call that changes the lengths was captured in a graph (or failed on its way): they
+    // may differ from the host's, which reads them back where it needs them.
     bool captured = false;
 };
 
@@ -2118,15 +2118,16 @@ int gonn_hip_kvcache8_append(gonn_kvcache8* h, const gonn_buf* k, const gonn_buf
         // The lengths that a captured append will meet are those of each replay.
         if (m < 0 || m > T || (capturing ? 0LL : h->len[b]) + m > c.Lmax) return GONN_E_INVALID;
     }
+    int rc;
     {
         ProfScope ps("kv8_append", s);
-        TRY(each_seqs8(c.B, counts, T, [&](const gonn::Seqs8& q) {
+        rc = each_seqs8(c.B, counts, T, [&](const gonn::Seqs8& q) {
             return gonn::launch_append8(c, k->ptr, v->ptr, k->dtype == GONN_BF16, T, q, s);
-        }));
+        });
     }
-    if (capturing) {
+    if (capturing || rc != GONN_OK) {  // after a failed launch some sequences may have grown
         h->captured = true;
-        return GONN_OK;
+        return rc;
     }
     for (int b = 0; b < c.B; b++) {
         h->len[b] += counts ? counts[b] : T;
@@ -2145,10 +2146,11 @@ int gonn_hip_kvcache8_truncate(gonn_kvcache8* h, const int* len, void* stream) {
         if (len[b] < 0 || len[b] > (capturing ? c.Lmax : h->len[b])) return GONN_E_INVALID;
         if (!capturing && len[b] < h->lo[b] && len[b] % gonn::kBlk8) return GONN_E_UNSUPPORTED;
     }
-    TRY(each_seqs8(c.B, len, 0, [&](const gonn::Seqs8& q) { return gonn::launch_truncate8(c, q, s); }));
-    if (capturing) {
+    const int rc =
+        each_seqs8(c.B, len, 0, [&](const gonn::Seqs8& q) { return gonn::launch_truncate8(c, q, s); });
+    if (capturing || rc != GONN_OK) {
         h->captured = true;
-        return GONN_OK;
+        return rc;
     }
     for (int b = 0; b < c.B; b++) {
         h->len[b] = len[b];

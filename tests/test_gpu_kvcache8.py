@@ -434,3 +434,24 @@ def test_many_sequences_of_different_lengths(T, dtype):
                    for b in some))
     for got in (o, og):
         check(torch.stack([got[b].cpu() for b in some]), torch.stack(ro), torch.stack(ra), f"{T} queries")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T", [1, 25, 60, 140])
+def test_outputs_given_and_neighbours_untouched(T, dtype):
+    """Outputs inside larger tensors; several splits, so that their join writes them."""
+    from gonn_amd import hip
+    B, Hq, H, D, n = 2, 2, 2, 64, 1900
+    k, v = (_rows(B, H, n, D, 140 + i).cuda() for i in range(2))
+    q = _rows(B, Hq, T, D, 142, dtype).cuda()
+    pad, flag = 256, -7.0
+    with hip.KVCache8(B, H, n, D) as c:
+        c.append(k, v)
+        want = (c.attend(q), *c.read(3, 500))
+        bigs = [torch.full((t.numel() + 2 * pad,), flag, dtype=t.dtype, device="cuda") for t in want]
+        o, rk, rv = (b[pad:-pad].view(t.shape) for b, t in zip(bigs, want))
+        assert c.attend(q, out=o) is o
+        c.read(3, 500, out=(rk, rv))
+        for b, x, w in zip(bigs, (o, rk, rv), want):
+            assert torch.equal(x, w)
+            assert (b[:pad] == flag).all() and (b[-pad:] == flag).all()

@@ -305,3 +305,35 @@ def test_offsets_past_32_bits():
     rg, rs, rn = ref.bwd(part(q), part(k), part(v), part(o), le, part(dO), scale, window, sinks)
     for name, x, r, s, m in zip(("dq", "dk", "dv"), grads, rg, rs, rn):
         ref.check(last(part(x)), last(r), last(s), name, last(m))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 70, 64), (8, 64, 32, 200, 200, 64), (4, 64, 16, 130, 140, 128)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_outputs_given_and_neighbours_untouched(shape, dtype):
+    """Outputs inside larger tensors: what lies before and behind them stays as it was, and
+    rows behind k's and v's last (infinite here) are not read."""
+    from gonn_amd import hip
+    B, H, Hkv, Sq, Sk, D = shape
+    q, k, v, dO = _data(shape, dtype, 41)
+    o, lse = hip.attn_window_fwd(q, k, v, window=30, sinks=3)
+    assert hip.attn_window_fwd(q, k, v, window=30, sinks=3, lse=False)[1] is None
+    want = (o, lse, *hip.attn_window_bwd(q, k, v, o, lse, dO, window=30, sinks=3))
+    pad, flag = 256, -7.0  # elements: keeps 16 bytes
+
+    def inside(t, fill=flag):
+        big = torch.full((t.numel() + 2 * pad,), fill, dtype=t.dtype, device="cuda")
+        x = big[pad:pad + t.numel()].view(t.shape)
+        x.copy_(t)
+        return big, x
+
+    ins = [inside(t, math.inf) for t in (q, k, v, dO)]
+    outs = [inside(torch.zeros_like(t)) for t in want]
+    q2, k2, v2, dO2 = (x for _, x in ins)
+    o2, lse2, dq, dk, dv = (x for _, x in outs)
+    got = hip.attn_window_fwd(q2, k2, v2, window=30, sinks=3, out=o2, lse_out=lse2)
+    assert got[0] is o2 and got[1] is lse2
+    hip.attn_window_bwd(q2, k2, v2, o2, lse2, dO2, window=30, sinks=3, out=(dq, dk, dv))
+    for (big, x), w in zip(outs, want):
+        assert torch.equal(x, w)
+        assert (big[:pad] == flag).all() and (big[-pad:] == flag).all()
