@@ -82,12 +82,15 @@ GONN_DEV int splits8(const Attend8& a, int nv) {
     return ns < a.nsplit ? ns : a.nsplit;
 }
 
-// Split and head of the workgroup whose turn is `us`, for rows of queries t0 ..
-// t1: of every 64 sequences those with the longest splits first. A workgroup streams 64
+// Split and head of the workgroup whose turn is `us`, for rows of queries t0 .. t1. Long
+// splits: of every 64 sequences those with the longest ones first. A workgroup streams 64
 // blocks for about 80 us, and one that starts last leaves the device idle for as long.
 // With the later splits, which only long sequences have, ahead of the first ones, short
 // sequences are left for the end. (2048 heads, 512 to 8192 positions, D 128, one row: 390
 // us in the order of the sequences, in splits of 64 blocks; 356 this way, in splits of 128.)
+// Splits of less than 32 blocks, 40 us, are taken as they come: finding the order is then
+// no small part of them (2048 heads, window 512: 70 us; ordered, by a loop over the
+// lanes, 75; window 100 37 and 42).
 struct Turn8 {
     int sp, len;  // split; the sequence's length
     size_t bh;    // its row of heads
@@ -95,23 +98,32 @@ struct Turn8 {
 GONN_DEV Turn8 turn_of(const Attend8& a, int us, int t0, int t1, int lane) {
     const Cache8& c = a.c;
     const int BH = c.B * c.H, order = us / BH, at = us - order * BH, place = at / c.H;
-    const int g0 = place & ~63, nb = c.B - g0 < 64 ? c.B - g0 : 64;
-    int key = -1, len = 0;
-    if (lane < nb) {
-        len = c.len[g0 + lane];
-        len = len < c.Lmax ? len : c.Lmax;
-        Blocks8 bs;
-        bs.init(len - a.T + t0, len - a.T + t1, a.window, a.sinks);
-        const int nv = bs.count(), ns = splits8(a, nv);
-        key = (ns ? (nv + ns - 1) / ns : 0) * 64 + 63 - lane;  // all different; under 2^31
+    int b = place, len = 0;
+    if (a.split >= 32) {
+        const int g0 = place & ~63;
+        int key = -1;
+        if (g0 + lane < c.B) {
+            len = c.len[g0 + lane];
+            len = len < c.Lmax ? len : c.Lmax;
+            Blocks8 bs;
+            bs.init(len - a.T + t0, len - a.T + t1, a.window, a.sinks);
+            const int nv = bs.count(), ns = splits8(a, nv);
+            key = (ns ? (nv + ns - 1) / ns : 0) * 64 + 63 - lane;  // all different; under 2^31
+        }
+        int before = 0;
+#pragma unroll
+        for (int j = 0; j < 64; j++) before += __builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(key >= 0 && before == (place & 63));
+        b = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
+        len = __builtin_amdgcn_readlane(len, b);
+        b += g0;
+    } else {
+        len = c.len[b];
+        len = __builtin_amdgcn_readfirstlane(len < c.Lmax ? len : c.Lmax);
     }
-    int before = 0;
-    for (int j = 0; j < nb; j++) before += __builtin_amdgcn_readlane(key, j) > key ? 1 : 0;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < nb && before == (place & 63));
-    const int at_lane = __builtin_amdgcn_readfirstlane(__builtin_ctzll(hit));
-    return {__builtin_amdgcn_readfirstlane(a.nsplit - 1 - order),
-            __builtin_amdgcn_readlane(len, at_lane),
-            (size_t)(g0 + at_lane) * c.H + __builtin_amdgcn_readfirstlane(at - place * c.H)};
+    b = __builtin_amdgcn_readfirstlane(b);
+    return {__builtin_amdgcn_readfirstlane(a.nsplit - 1 - order), len,
+            (size_t)b * c.H + __builtin_amdgcn_readfirstlane(at - place * c.H)};
 }
 
 GONN_DEV bool sees8(int i, int j, int window, int sinks) {
